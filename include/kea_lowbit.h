@@ -75,7 +75,8 @@ enum {
 enum {
     KEA_DEVERR_TIMEOUT = 1,      /* an mbarrier wait exceeded its bound */
     KEA_DEVERR_TAIL_BITS = 2,    /* prepare: nonzero padding bits past K */
-    KEA_DEVERR_TERNARY_11 = 4    /* prepare: a 2-bit field holds the unused pattern 0b11 */
+    KEA_DEVERR_TERNARY_11 = 4,   /* prepare: a 2-bit field holds the unused pattern 0b11 */
+    KEA_DEVERR_INDEX = 8         /* beam_reorder: a parent outside the hypotheses */
 };
 
 /*
@@ -313,6 +314,126 @@ typedef struct KeaAttentionDesc {
 } KeaAttentionDesc;
 
 int kea_lowbit_rel_attention(const KeaAttentionDesc *desc, void *stream);
+
+/* Element types of the operators below. */
+enum { KEA_TYPE_F32 = 0, KEA_TYPE_F16 = 1, KEA_TYPE_BF16 = 2 };
+
+/* One 8-bit linear map: INT8 activations with a scale per token times INT8 weights with a scale per channel,
+ *   acc[m, n] = sum_k q[m, k] * w[n, k]                                  (exact INT32)
+ *   v         = bias ? fma(RN(acc) * qs[m], alpha[n], bias[n]) : (RN(acc) * qs[m]) * alpha[n],  then SiLU if KEA_INT8_SILU
+ *   y[m, n]   = residual ? residual[m, n] + residual_scale * v : v       (FP32, rounded once to y_type)
+ * with one IEEE FP32 rounding per operation, as kea_lowbit_gemm. For layers kept at 8 bits (a joint network, layers an
+ * export leaves unpacked); the weights are used as they are, row-major, without a layout pass. k <= 131071, where no sum
+ * can leave INT32. q and w: 16-byte aligned, row strides multiples of 16; columns >= k are never used. */
+typedef struct KeaInt8Desc {
+    const int8_t *q;          /* [m][ldq] */
+    int64_t ldq;
+    const float *qs;          /* [m] */
+    const int8_t *w;          /* [n][ldw] */
+    int64_t ldw;
+    const float *alpha;       /* [n] */
+    const float *bias;        /* [n] or NULL */
+    void *y;                  /* [m][ldy] of y_type */
+    int64_t ldy;
+    const void *residual;     /* [m][ld_residual] of y_type, or NULL; may be y itself */
+    int64_t ld_residual;
+    int32_t *acc;             /* INT32 [m][ld_acc] sums, or NULL */
+    int64_t ld_acc;
+    float residual_scale;
+    int32_t m, n, k;          /* m 0 is a no-op */
+    int32_t y_type;           /* KEA_TYPE_* */
+    int32_t flags;            /* KEA_INT8_* */
+    int32_t kernel;           /* 0: chosen by the shape; else KEA_INT8_KERNEL_* */
+    uint32_t *error_word;     /* device word OR-ed with KEA_DEVERR_* bits, or NULL for the library's own */
+} KeaInt8Desc;
+
+enum { KEA_INT8_SILU = 1, KEA_INT8_PDL = 2 };
+enum { KEA_INT8_KERNEL_REG = 1 };
+
+int kea_lowbit_int8_gemm(const KeaInt8Desc *desc, void *stream);
+
+/* The step between two blocks of a residual network, in one pass over its rows:
+ *   u = post(y)                          (y: the block's output; LayerNorm, root-mean-square norm or nothing)
+ *   r = x + scale * act(gate) * u        (the residual stream; x and r of x_type, r may be x itself)
+ *   h = pre(r)                           (the next block's norm, of r before its rounding; h of h_type and / or INT8 codes)
+ * post and pre take FP32 weights and biases [d] (bias NULL: none); LayerNorm is (v - mean) / sqrt(var + eps), the
+ * root-mean-square norm v / sqrt(mean(v^2) + eps). gate (y_type, or NULL): value (row m, column i) at
+ * gate + (m / frames) * gate_clip_stride + (m % frames) * gate_row_stride + i, so 0 strides share it; act: as is, or the
+ * logistic function. q / qs: INT8 codes and one scale per row of h, as kea_lowbit_quantize forms one part (columns d ..
+ * ldq - 1 written as 0). All arithmetic is FP32. d <= 16384. h and q may not overlap x, y or the gate. */
+typedef struct KeaResidualNormDesc {
+    const void *x, *y, *gate;
+    int64_t ldx, ldy;             /* row strides in elements */
+    int64_t gate_clip_stride, gate_row_stride;
+    int32_t frames;               /* rows per clip (>= 1) */
+    int32_t gate_act;             /* KEA_GATE_* */
+    int32_t x_type, y_type, h_type;
+    int32_t post, pre;            /* KEA_NORM_* */
+    float scale, post_eps, pre_eps;
+    const float *post_weight, *post_bias, *pre_weight, *pre_bias;
+    void *r, *h;                  /* h NULL: only the codes */
+    int64_t ldr, ldh;
+    int8_t *q;                    /* NULL: no codes */
+    int32_t ldq;
+    float *qs;                    /* [m] */
+    int32_t m, d;                 /* m 0 is a no-op */
+    int32_t flags;                /* KEA_RNORM_* */
+} KeaResidualNormDesc;
+
+enum { KEA_NORM_NONE = 0, KEA_NORM_LAYER = 1, KEA_NORM_RMS = 2 };
+enum { KEA_GATE_NONE = 0, KEA_GATE_SIGMOID = 1 };
+enum { KEA_RNORM_PDL = 1 };
+
+int kea_lowbit_residual_norm(const KeaResidualNormDesc *desc, void *stream);
+
+/* One step of a beam search: the `width` best continuations of every clip's hypotheses.
+ *   c[b, k, v] = scores[b, k] + log_softmax(logits[b, k, :])[v]      (FP32), flat index k * vocab + v;
+ * an ended hypothesis offers only the label `end`, at its own score. The continuations come in descending order, equal
+ * ones by their flat index; within a hypothesis the logits themselves are compared. A logit that is -inf or not a number
+ * is masked; a hypothesis whose score or log-sum is not finite (no label left, a logit of +inf) offers nothing. What is
+ * not offered counts as -inf: where fewer than `width` are offered, the places left take such continuations by their flat
+ * index, with score -inf.
+ * logits: (b, k, v) at logits + b * ld_clip + k * ld_beam + v, any stride; scores FP32 [clips][beams]. beams and width <= 32,
+ * width <= beams * vocab < 2^31. The outputs may not overlap the inputs. */
+typedef struct KeaBeamDesc {
+    const void *logits;
+    int64_t ld_clip, ld_beam;     /* elements */
+    const float *scores;
+    const uint8_t *ended;         /* [clips][beams], nonzero: ended; or NULL */
+    float *out_scores;            /* [clips][width] */
+    int32_t *parents, *labels;    /* [clips][width] */
+    uint8_t *out_ended;           /* [clips][width] (the parent has ended, or the label is `end`), or NULL */
+    int32_t clips, beams, vocab, width;   /* clips 0 is a no-op */
+    int32_t end;                  /* the label that ends a hypothesis, or -1 */
+    int32_t logits_type;          /* KEA_TYPE_* */
+    int32_t flags;                /* KEA_BEAM_* */
+} KeaBeamDesc;
+
+enum { KEA_BEAM_PDL = 1 };
+
+int kea_lowbit_beam_select(const KeaBeamDesc *desc, void *stream);
+
+/* The states of the chosen hypotheses, for up to KEA_REORDER_MAX buffers in one launch: of every buffer, and every group g
+ * of it (layers, for instance),  dst[g, b, w] = src[g, b, parents[b, w]],  rows of row_bytes bytes at byte strides. A
+ * parent outside [0, beams) leaves a row of zeros and sets KEA_DEVERR_INDEX in the error word. dst may not overlap src.
+ * `items` (desc->count of them) is host memory, read during the call. */
+#define KEA_REORDER_MAX 32
+typedef struct KeaReorderItem {
+    const void *src;
+    void *dst;
+    int64_t src_group, src_clip, src_beam;   /* byte strides */
+    int64_t dst_group, dst_clip, dst_beam;
+    int64_t row_bytes;
+    int32_t groups;               /* >= 1 */
+} KeaReorderItem;
+typedef struct KeaReorderDesc {
+    const int32_t *parents;       /* [clips][width] */
+    int32_t count, clips, beams, width;
+    int32_t flags;                /* KEA_BEAM_* */
+    uint32_t *error_word;         /* device word, or NULL for the library's own */
+} KeaReorderDesc;
+
+int kea_lowbit_beam_reorder(const KeaReorderDesc *desc, const KeaReorderItem *items, void *stream);
 
 /* Reads and clears the library's own device error word on the current device. Synchronizes the device. */
 int kea_lowbit_read_error(uint32_t *out);

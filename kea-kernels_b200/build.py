@@ -9,14 +9,16 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 ROOT = HERE.parent
 CSRC = HERE / "csrc"
 OUT = HERE / "kea_kernels" / "libkea_lowbit.so"
-SOURCES = [CSRC / "kea_lowbit.cu"]
-HEADERS = sorted(CSRC.glob("*.cuh")) + [ROOT / "include" / "kea_lowbit.h"]
+SOURCES = [CSRC / f"{name}.cu" for name in ("kea_lowbit", "int8_gemm", "residual_norm", "beam")]
+HEADERS = sorted(CSRC.glob("*.cuh")) + [CSRC / "host.h", ROOT / "include" / "kea_lowbit.h"]
 
 
 def nvcc() -> str:
@@ -26,27 +28,40 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found: set NVCC or add the CUDA toolkit to PATH")
 
 
-def command() -> list[str]:
+def compile_command(source: Path, obj: Path) -> list[str]:
     return [nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-            "-fmad=false", "-Xptxas", "-v", f"-I{ROOT / 'include'}", "-Xcompiler", "-fPIC,-O2", "-shared",
-            "-o", str(OUT), *map(str, SOURCES)]
+            "-fmad=false", "-Xptxas", "-v", f"-I{ROOT / 'include'}", "-Xcompiler", "-fPIC,-O2", "-c",
+            "-o", str(obj), str(source)]
+
+
+def link_command(objects: list[Path]) -> list[str]:
+    return [nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", str(OUT), *map(str, objects)]
+
+
+def newest_input(source: Path) -> float:
+    return max(p.stat().st_mtime for p in [source, *HEADERS, Path(__file__)])
 
 
 def stale() -> bool:
-    if not OUT.exists():
-        return True
-    built = OUT.stat().st_mtime
-    return any(p.stat().st_mtime > built for p in SOURCES + HEADERS + [Path(__file__)])
+    return not OUT.exists() or any(newest_input(s) > OUT.stat().st_mtime for s in SOURCES)
+
+
+def run(cmd: list[str]) -> str:
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+    return res.stderr
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compiles the sources side by side into a temporary folder and links them."""
     if force or stale():
-        cmd = command()
-        res = subprocess.run(cmd, capture_output=True, text=True)
-        if res.returncode != 0:
-            raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+        with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(len(SOURCES)) as pool:
+            objects = [Path(tmp) / f"{s.stem}.o" for s in SOURCES]
+            logs = list(pool.map(run, map(compile_command, SOURCES, objects)))
+            logs.append(run(link_command(objects)))
         if verbose:
-            print(res.stderr)
+            print("".join(logs))
     return OUT
 
 

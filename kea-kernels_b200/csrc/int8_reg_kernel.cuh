@@ -1,0 +1,144 @@
+// int8_reg_kernel.cuh - the 8-bit GEMM for few tokens: warp-level tensor-core MMAs (mma.sync m16n8k32, INT8 x INT8 ->
+// INT32) on operands loaded straight from global memory into registers.
+//
+// With a handful of tokens the weights are nearly all that is read (N x K bytes for 2 M N K operations), and a launch
+// lasts a few microseconds: what counts is that every byte is requested at once and that nothing is set up first. So no
+// shared-memory staging, no barriers before the sums: a warp asks for its operands a few steps ahead, in 16-byte loads.
+//
+// Operands. The weights are the MMA's A operand (16 channels x 32 k), the tokens B (32 k x 8 rows). An integer sum does
+// not depend on the order of its terms as long as both operands use the same one, so k is walked in steps of 64 (two
+// MMAs): lane (g, t) (g = lane / 4, t = lane % 4) holds bytes 16 t .. 16 t + 15 of rows g and g + 8 of its 16 channels and of
+// token row g; bytes 0-3 / 4-7 of a 16-byte group are the first MMA's two k registers, 8-11 / 12-15 the second's.
+//
+// Work split. A CTA = 8 warps owns CN channels x 8 RG tokens; the warps are KS slices of K x (8 / KS) groups of 16 CG
+// channels. The slices' INT32 sums meet in shared memory and are added in slice order (exact), then finished.
+// Weights do not depend on the previous kernel of the stream: the first loads are issued before griddepcontrol.wait.
+#pragma once
+
+#include "int8_epilogue.cuh"
+
+namespace kea {
+
+constexpr int kI8RegThreads = 256, kI8RegWarps = 8, kI8RegPad = 4;
+
+__host__ __device__ inline int i8reg_smem_bytes(int ks, int rows, int cn) { return ks * rows * (cn + kI8RegPad) * 4; }
+
+KEA_DEVI void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 bytes at column k of a row of K valid bytes (16-byte aligned): zeros past K, and nothing past K is read.
+template <bool CONST>
+KEA_DEVI uint4 load_codes(const int8_t *row, int k, int K) {
+    if (row == nullptr || k >= K) return make_uint4(0u, 0u, 0u, 0u);
+    const uint4 *p = reinterpret_cast<const uint4 *>(row + k);
+    if (k + 16 <= K) return CONST ? __ldg(p) : *p;
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 15; ++i)
+        if (k + i < K) w[i >> 2] |= (uint32_t)(uint8_t)row[k + i] << (8 * (i & 3));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T, int CG, int RG, int D>
+__global__ void __launch_bounds__(kI8RegThreads, 2) int8_gemm_reg_kernel(const Int8Args a, int KS) {
+    extern __shared__ __align__(16) int rsm[];
+    grid_launch_dependents();
+    constexpr int R = 8 * RG;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
+    const int CW = kI8RegWarps / KS, kw = warp % KS, cw = warp / KS;
+    const int CN = 16 * CG * CW;
+    const int c0 = blockIdx.x * CN, m0 = blockIdx.y * R;
+    const int steps = (a.K + 63) / 64, per = (steps + KS - 1) / KS;
+    const int s0 = min(steps, kw * per), s1 = min(steps, s0 + per);
+
+    const int8_t *wrow[CG][2], *qrow[RG];
+#pragma unroll
+    for (int c = 0; c < CG; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int n = c0 + 16 * (cw * CG + c) + g + 8 * h;
+            wrow[c][h] = n < a.N ? a.w + (long long)n * a.ldw : nullptr;
+        }
+#pragma unroll
+    for (int r = 0; r < RG; ++r) {
+        const int m = m0 + 8 * r + g;
+        qrow[r] = m < a.M ? a.q + (long long)m * a.ldq : nullptr;
+    }
+
+    uint4 wr[D][CG][2], br[D][RG];
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+#pragma unroll
+        for (int c = 0; c < CG; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                wr[d][c][h] = load_codes<true>(wrow[c][h], s0 + d < s1 ? 64 * (s0 + d) + 16 * t : a.K, a.K);
+    grid_dependency_wait();
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+#pragma unroll
+        for (int r = 0; r < RG; ++r)
+            br[d][r] = load_codes<false>(qrow[r], s0 + d < s1 ? 64 * (s0 + d) + 16 * t : a.K, a.K);
+
+    int acc[CG][RG][4];
+#pragma unroll
+    for (int c = 0; c < CG; ++c)
+#pragma unroll
+        for (int r = 0; r < RG; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[c][r][i] = 0;
+
+    for (int base = s0; base < s1; base += D) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            const int s = base + d;
+            if (s >= s1) break;
+#pragma unroll
+            for (int c = 0; c < CG; ++c)
+#pragma unroll
+                for (int r = 0; r < RG; ++r) {
+                    mma_s8(acc[c][r], wr[d][c][0].x, wr[d][c][1].x, wr[d][c][0].y, wr[d][c][1].y, br[d][r].x, br[d][r].y);
+                    mma_s8(acc[c][r], wr[d][c][0].z, wr[d][c][1].z, wr[d][c][0].w, wr[d][c][1].w, br[d][r].z, br[d][r].w);
+                }
+            const int k = s + D < s1 ? 64 * (s + D) + 16 * t : a.K;   // this slot's next step
+#pragma unroll
+            for (int c = 0; c < CG; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) wr[d][c][h] = load_codes<true>(wrow[c][h], k, a.K);
+#pragma unroll
+            for (int r = 0; r < RG; ++r) br[d][r] = load_codes<false>(qrow[r], k, a.K);
+        }
+    }
+
+    // the D fragment: channels g / g + 8, token rows 2 t / 2 t + 1
+    const int ld = CN + kI8RegPad;
+    int *part = rsm + kw * R * ld;
+#pragma unroll
+    for (int c = 0; c < CG; ++c)
+#pragma unroll
+        for (int r = 0; r < RG; ++r) {
+            const int ch = 16 * (cw * CG + c) + g, row = 8 * r + 2 * t;
+            part[row * ld + ch] = acc[c][r][0];
+            part[(row + 1) * ld + ch] = acc[c][r][1];
+            part[row * ld + ch + 8] = acc[c][r][2];
+            part[(row + 1) * ld + ch + 8] = acc[c][r][3];
+        }
+    __syncthreads();
+    const bool has_bias = a.bias != nullptr;
+    for (int i = threadIdx.x; i < R * CN; i += kI8RegThreads) {
+        const int row = i / CN, ch = i - row * CN, m = m0 + row, n = c0 + ch;
+        if (m >= a.M || n >= a.N) continue;
+        int v = 0;
+        for (int w = 0; w < KS; ++w) v += rsm[(w * R + row) * ld + ch];
+        if (a.acc) a.acc[(long long)m * a.ld_acc + n] = v;
+        int8_store<T>(a, m, n, int8_value(v, a.qs[m], __ldg(a.alpha + n), has_bias, has_bias ? __ldg(a.bias + n) : 0.f,
+                                          a.silu != 0));
+    }
+}
+
+}  // namespace kea

@@ -9,6 +9,7 @@
 #include <mutex>
 
 #include "kea_lowbit.h"
+#include "host.h"
 #include "gemm_kernel.cuh"
 #include "gemm_pair_kernel.cuh"
 #include "gemm_pair_ws_kernel.cuh"
@@ -41,6 +42,7 @@ struct DeviceState {
     int status = KEA_OK;
     int sms = kSmsB200;
     void *noalloc_scratch = nullptr;   // device address of g_noalloc_scratch on this device
+    void *error_word = nullptr;        // device address of kea::g_device_error on this device
 };
 DeviceState g_devices[kMaxDevices];
 std::mutex g_mutex;
@@ -50,9 +52,7 @@ std::mutex g_mutex;
 // from cudaGetSymbolAddress, looked up in the one-time set-up of each device with that device current.
 static __device__ __align__(256) int g_noalloc_scratch[KEA_NOALLOC_SCRATCH_BYTES / sizeof(int)];
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+using kea_host::EncodeTiledFn;
 EncodeTiledFn g_encode = nullptr;
 
 // One-time per-device set-up: capability check, kernel attributes and the no-allocation scratch address. Nothing here
@@ -159,13 +159,30 @@ int device_setup(int *device_out, void *stream, bool check_capture = true) {
         void *addr = nullptr;
         if (cudaGetSymbolAddress(&addr, g_noalloc_scratch) != cudaSuccess || !addr) status = KEA_ERR_CUDA;
         st.noalloc_scratch = addr;
+        if (cudaGetSymbolAddress(&addr, kea::g_device_error) != cudaSuccess || !addr) status = KEA_ERR_CUDA;
+        st.error_word = addr;
     }
+    if (status == KEA_OK) status = kea_host::setup_int8_gemm();
     if (status != KEA_OK) cudaGetLastError();
     st.status = status;
     st.sms = sms > 0 ? sms : kSmsB200;
     st.ready = true;
     return status;
 }
+
+}  // namespace
+
+int kea_host::device(Device *out, void *stream) {
+    const int st = device_setup(&out->index, stream);
+    if (st != KEA_OK) return st;
+    const DeviceState &d = g_devices[out->index];
+    out->sms = d.sms;
+    out->error_word = static_cast<uint32_t *>(d.error_word);
+    out->encode = g_encode;
+    return KEA_OK;
+}
+
+namespace {
 
 // ---- configuration ---------------------------------------------------------------------------------------
 // Per-stage bytes of the three shared-memory regions (activation tiles, expanded weights, packed codes).

@@ -1,0 +1,46 @@
+// operator_common.cuh - device pieces shared by the 8-bit GEMM, the residual-norm and the beam-search kernels: element
+// types, their conversions and the error report.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "kea_lowbit.h"
+#include "ptx.cuh"
+
+namespace kea {
+
+template <typename T> struct TypeCode;
+template <> struct TypeCode<float> { static constexpr int value = KEA_TYPE_F32; };
+template <> struct TypeCode<__half> { static constexpr int value = KEA_TYPE_F16; };
+template <> struct TypeCode<__nv_bfloat16> { static constexpr int value = KEA_TYPE_BF16; };
+
+KEA_DEVI float to_float(float v) { return v; }
+KEA_DEVI float to_float(__half v) { return __half2float(v); }
+KEA_DEVI float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T> KEA_DEVI T from_float(float v);
+template <> KEA_DEVI float from_float<float>(float v) { return v; }
+template <> KEA_DEVI __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> KEA_DEVI __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Two values rounded to nearest even and packed, `lo` in the lower half.
+template <typename T> KEA_DEVI uint32_t pack2(float lo, float hi);
+template <> KEA_DEVI uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> KEA_DEVI uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <typename T> KEA_DEVI float2 unpack2(uint32_t w);
+template <> KEA_DEVI float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+template <> KEA_DEVI float2 unpack2<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+
+KEA_DEVI void report_error(uint32_t *word, uint32_t bits) { atomicOr(word, bits); }
+
+}  // namespace kea
