@@ -4,6 +4,7 @@
 
 #include "host.h"
 #include "int8_reg_kernel.cuh"
+#include "int8_tile_kernel.cuh"
 #include "kea_lowbit.h"
 
 namespace {
@@ -12,11 +13,11 @@ using kea_host::aligned;
 using kea_host::ceil_div;
 
 constexpr int kMaxK = 131071;   // 128 * 128 * k < 2^31
-constexpr int kRegMaxSmem = 64 * 1024;
+constexpr int kMaxDynSmem = 227 * 1024 - 1024;   // the kernels' static shared memory is a few hundred bytes
 
 int validate(const KeaInt8Desc *d) {
     if (!d || d->m < 0 || d->n < 1 || d->k < 1 || d->y_type < KEA_TYPE_F32 || d->y_type > KEA_TYPE_BF16 ||
-        (d->flags & ~(KEA_INT8_SILU | KEA_INT8_PDL)) || d->kernel < 0 || d->kernel > KEA_INT8_KERNEL_REG)
+        (d->flags & ~(KEA_INT8_SILU | KEA_INT8_PDL)) || d->kernel < 0 || d->kernel > KEA_INT8_KERNEL_PAIR)
         return KEA_ERR_INVALID_VALUE;
     if (d->m == 0) return KEA_OK;
     if (!d->q || !d->qs || !d->w || !d->alpha || !d->y || d->ldq < d->k || d->ldw < d->k || d->ldy < d->n)
@@ -94,9 +95,99 @@ cudaError_t launch_reg(const kea::Int8Args &a, int sms, bool pdl, void *stream) 
     return launch_reg_as<T, 2, 4, 2>(a, a.K >= 512 ? 4 : 1, pdl, stream);
 }
 
+// ---- tcgen05 kernels -----------------------------------------------------------------------------------------------
+// Row-major matrix of 8-bit codes -> boxes of 128 bytes of K x `rows` rows, 128-byte swizzle; zeros outside.
+bool map_codes(const kea_host::Device &dev, CUtensorMap *map, const int8_t *p, long long ld, int rows_total, int k, int rows) {
+    const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows_total};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld};
+    const cuuint32_t box[2] = {(cuuint32_t)kea::kI8K, (cuuint32_t)rows}, step[2] = {1, 1};
+    return dev.encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(p), dims, strides, box, step,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The output as boxes of 32 rows x 128 bytes, where its rows are 16-byte aligned.
+bool map_output(const kea_host::Device &dev, CUtensorMap *map, const kea::Int8Args &a) {
+    const int size = a.y_type == KEA_TYPE_F32 ? 4 : 2;
+    if (!aligned(a.y, 16) || (a.ldy * size) % 16) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)a.N, (cuuint64_t)a.M};
+    const cuuint64_t strides[1] = {(cuuint64_t)(a.ldy * size)};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), 32}, step[2] = {1, 1};
+    const CUtensorMapDataType type = a.y_type == KEA_TYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : a.y_type == KEA_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return dev.encode(map, type, 2, a.y, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int CTAS, int BN>
+int stages_for(int kbs, int tiles_per_worker) {
+    int s = kea::kI8MaxStages;
+    while (s > 2 && kea::Int8Tile<CTAS, BN>::smem(s) > kMaxDynSmem) --s;
+    return std::max(2, std::min<int>(s, kbs * tiles_per_worker));
+}
+
+template <typename T, bool SILU, int CTAS, int BN>
+cudaError_t launch_tile_as(const kea_host::Device &dev, const kea::Int8Args &a, bool pdl, void *stream) {
+    using Tile = kea::Int8Tile<CTAS, BN>;
+    kea::Int8TileArgs p{};
+    p.a = a;
+    p.n_tiles = ceil_div(a.N, BN);
+    const long long tiles = (long long)p.n_tiles * ceil_div(a.M, 128 * CTAS);
+    if (tiles >= (1LL << 30)) return cudaErrorInvalidValue;
+    p.tiles = (int)tiles;
+    p.kbs = ceil_div(a.K, kea::kI8K);
+    const int workers = std::min(p.tiles, std::max(1, dev.sms / CTAS));
+    p.stages = stages_for<CTAS, BN>(p.kbs, ceil_div(p.tiles, workers));
+    CUtensorMap qmap, wmap, ymap{};
+    if (!map_codes(dev, &qmap, a.q, a.ldq, a.M, a.K, 128) || !map_codes(dev, &wmap, a.w, a.ldw, a.N, a.K, BN / CTAS))
+        return cudaErrorInvalidValue;
+    const size_t size = sizeof(T);
+    p.tma_store = map_output(dev, &ymap, a) ? 1 : 0;
+    p.res_vec = a.res && aligned(a.res, 16) && (a.ld_res * (long long)size) % 16 == 0 && ((size_t)a.N * size) % 16 == 0;
+    const Launch l(dim3((unsigned)(workers * CTAS), 1, 1), Tile::THREADS, Tile::smem(p.stages), stream, pdl, CTAS);
+    return cudaLaunchKernelEx(&l.cfg, kea::int8_gemm_tile_kernel<T, SILU, CTAS, BN>, qmap, wmap, ymap, p);
+}
+
+template <typename T>
+cudaError_t launch_typed(const kea_host::Device &dev, const kea::Int8Args &a, int kernel, bool pdl, void *stream) {
+    switch (kernel) {
+        case KEA_INT8_KERNEL_TILE64:
+            return a.silu ? launch_tile_as<T, true, 1, 64>(dev, a, pdl, stream) : launch_tile_as<T, false, 1, 64>(dev, a, pdl, stream);
+        case KEA_INT8_KERNEL_TILE128:
+            return a.silu ? launch_tile_as<T, true, 1, 128>(dev, a, pdl, stream) : launch_tile_as<T, false, 1, 128>(dev, a, pdl, stream);
+        case KEA_INT8_KERNEL_PAIR:
+            return a.silu ? launch_tile_as<T, true, 2, 256>(dev, a, pdl, stream) : launch_tile_as<T, false, 2, 256>(dev, a, pdl, stream);
+        default: return launch_reg<T>(a, dev.sms, pdl, stream);
+    }
+}
+
+int choose(const kea::Int8Args &a, int sms) {
+    if (a.M <= 64) return KEA_INT8_KERNEL_REG;
+    if ((long long)ceil_div(a.M, 256) * ceil_div(a.N, 256) >= sms / 2) return KEA_INT8_KERNEL_PAIR;
+    if ((long long)ceil_div(a.M, 128) * ceil_div(a.N, 128) >= sms / 2) return KEA_INT8_KERNEL_TILE128;
+    return KEA_INT8_KERNEL_TILE64;
+}
+
+template <typename T, bool SILU>
+bool attributes() {
+    const auto set = [](const void *kernel) {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynSmem) == cudaSuccess;
+    };
+    return set((const void *)kea::int8_gemm_tile_kernel<T, SILU, 1, 64>) &&
+           set((const void *)kea::int8_gemm_tile_kernel<T, SILU, 1, 128>) &&
+           set((const void *)kea::int8_gemm_tile_kernel<T, SILU, 2, 256>);
+}
+
 }  // namespace
 
-int kea_host::setup_int8_gemm() { return KEA_OK; }
+int kea_host::setup_int8_gemm() {
+    return attributes<float, false>() && attributes<float, true>() && attributes<__half, false>() && attributes<__half, true>() &&
+                   attributes<__nv_bfloat16, false>() && attributes<__nv_bfloat16, true>()
+               ? KEA_OK
+               : KEA_ERR_CUDA;
+}
 
 extern "C" int kea_lowbit_int8_gemm(const KeaInt8Desc *d, void *stream) {
     const int v = validate(d);
@@ -106,10 +197,11 @@ extern "C" int kea_lowbit_int8_gemm(const KeaInt8Desc *d, void *stream) {
     if (st != KEA_OK) return st;
     const kea::Int8Args a = arguments(d, dev);
     const bool pdl = (d->flags & KEA_INT8_PDL) != 0;
-    if (ceil_div(a.M, 32) > 65535) return KEA_ERR_UNSUPPORTED;
-    const cudaError_t e = a.y_type == KEA_TYPE_F32   ? launch_reg<float>(a, dev.sms, pdl, stream)
-                          : a.y_type == KEA_TYPE_F16 ? launch_reg<__half>(a, dev.sms, pdl, stream)
-                                                     : launch_reg<__nv_bfloat16>(a, dev.sms, pdl, stream);
+    const int kernel = d->kernel ? d->kernel : choose(a, dev.sms);
+    if (kernel == KEA_INT8_KERNEL_REG && ceil_div(a.M, 32) > 65535) return KEA_ERR_UNSUPPORTED;
+    const cudaError_t e = a.y_type == KEA_TYPE_F32   ? launch_typed<float>(dev, a, kernel, pdl, stream)
+                          : a.y_type == KEA_TYPE_F16 ? launch_typed<__half>(dev, a, kernel, pdl, stream)
+                                                     : launch_typed<__nv_bfloat16>(dev, a, kernel, pdl, stream);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return KEA_ERR_CUDA;

@@ -1,0 +1,409 @@
+// int8_tile_kernel.cuh - the 8-bit GEMM on the tcgen05 tensor cores: both operands by TMA, INT32 accumulators in tensor
+// memory, persistent CTAs (CTAS = 1) or CTA pairs (CTAS = 2, tcgen05 cta_group::2).
+//
+// A tile is 128 CTAS tokens x BN channels. A CTA holds 128 token rows of it and BN / CTAS channel rows; for a pair the even
+// CTA issues the MMAs of both (M 256 x N 256 x K 32), each SM reading only its own shared memory, so a byte of either
+// operand serves 256 products. K goes by in blocks of 128 bytes (rows of 128 bytes in the 128-byte swizzle, K-major);
+// rows and columns past M, N and K are filled with zeros by the copies. Tensor memory holds two accumulators, so the
+// epilogue of one tile runs while the MMAs of the next fill the other.
+//
+// Warps: 0 producer (one lane: TMA loads); 1 tensor memory and MMA issue; 2 .. epilogue, warp pair (w % 4) reading the
+// 32 tensor-memory lanes it may, in HALVES column halves: TMEM -> scales, bias, SiLU, skip connection -> boxes of 32 rows
+// x 128 bytes staged in shared memory (128-byte swizzle) -> TMA stores, or row-wise stores where the output's rows are
+// not 16-byte aligned. Every wait is bounded; one that runs out is reported in the error word and the kernel ends.
+#pragma once
+
+#include "int8_epilogue.cuh"
+
+namespace kea {
+
+constexpr int kI8K = 128;                 // bytes of K per stage
+constexpr uint32_t kI8Half = 128u * kI8K; // 128 rows of a stage
+constexpr uint32_t kI8Box = 4096;         // one output box: 32 rows x 128 bytes
+constexpr int kI8MaxStages = 8;
+
+template <int CTAS, int BN>
+struct Int8Tile {
+    static constexpr int HALVES = BN >= 128 ? 2 : 1, EPI_WARPS = 4 * HALVES, THREADS = 64 + 32 * EPI_WARPS;
+    static constexpr int CW = BN / HALVES;                                // columns per epilogue warp
+    static constexpr int BUFS = 2;                                        // staging boxes per epilogue warp
+    static constexpr uint32_t B_BYTES = (uint32_t)(BN / CTAS) * kI8K, STAGE = kI8Half + B_BYTES;
+    static constexpr uint32_t STAGING = EPI_WARPS * BUFS * kI8Box, CONSTS = EPI_WARPS * CW * 8u;
+    static constexpr uint32_t smem(int stages) { return 1024u + (uint32_t)stages * STAGE + STAGING + CONSTS; }
+};
+
+struct Int8TileArgs {
+    Int8Args a;
+    int n_tiles, tiles, kbs, stages;
+    int tma_store, res_vec;
+};
+
+KEA_DEVI void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+
+KEA_DEVI void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    tmem_ld16(taddr, *reinterpret_cast<uint32_t(*)[16]>(&v[0]));
+    tmem_ld16(taddr + 16u, *reinterpret_cast<uint32_t(*)[16]>(&v[16]));
+}
+
+// The skip connection's 32 rows x 128 bytes in front of a box, read row-wise into the staging space (swizzled).
+template <typename T>
+KEA_DEVI void int8_stage_residual(const Int8Args &a, uint32_t stg, int row0, int n0) {
+    const int lane = threadIdx.x & 31, piece = lane & 7;
+    constexpr int E = 16 / sizeof(T);
+    const int n = n0 + piece * E;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3), t = row0 + r;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (t < a.M && n < a.N)
+            v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.res) + (long long)t * a.ld_res + n);
+        st_shared16(stg + (uint32_t)r * 128u + (uint32_t)((piece ^ (r & 7)) << 4), v.x, v.y, v.z, v.w);
+    }
+}
+
+// A staged box written row by row: one row's 128 bytes per warp store.
+template <typename T>
+KEA_DEVI void int8_store_rows(const Int8Args &a, uint32_t stg, int row0, int n0) {
+    const int lane = threadIdx.x & 31;
+    for (int r = 0; r < 32 && row0 + r < a.M; ++r) {
+        uint32_t w;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(stg + (uint32_t)r * 128u + (uint32_t)(((lane >> 2) ^ (r & 7)) << 4) + (uint32_t)(lane & 3) * 4u) : "memory");
+        T *dst = static_cast<T *>(a.y) + (long long)(row0 + r) * a.ldy;
+        if constexpr (sizeof(T) == 4) {
+            if (n0 + lane < a.N) reinterpret_cast<uint32_t *>(dst)[n0 + lane] = w;
+        } else {
+            uint16_t *d16 = reinterpret_cast<uint16_t *>(dst);
+            if (n0 + 2 * lane < a.N) d16[n0 + 2 * lane] = (uint16_t)w;
+            if (n0 + 2 * lane + 1 < a.N) d16[n0 + 2 * lane + 1] = (uint16_t)(w >> 16);
+        }
+    }
+}
+
+// One epilogue warp's 32 rows x CW columns of a finished tile. `release` hands the accumulator back.
+template <typename T, bool SILU, int CW, int BUFS, typename Release>
+KEA_DEVI void int8_epilogue_tile(const Int8TileArgs &p, const CUtensorMap *ymap, uint32_t taddr, uint32_t stg0, uint32_t consts,
+                                 int row0, int n0, float sq, int &box, Release release) {
+    const Int8Args &a = p.a;
+    const int lane = threadIdx.x & 31, t = row0 + lane;
+    constexpr int NC = 128 / (int)sizeof(T), SUBS = NC / 32;
+    const bool has_bias = a.bias != nullptr;
+    uint32_t v[32];
+#pragma unroll 1
+    for (int b = 0; b < CW / NC; ++b, ++box) {
+        const uint32_t stg = stg0 + (uint32_t)(box % BUFS) * kI8Box;
+        if (lane == 0) {   // the store that last read this space is done with it
+            if constexpr (BUFS == 2) bulk_wait_group_read1();
+            else bulk_wait_group_read0();
+        }
+        __syncwarp();
+        const int nb = n0 + b * NC;
+        if (a.res && p.res_vec) {
+            int8_stage_residual<T>(a, stg, row0, nb);
+            __syncwarp();
+        }
+#pragma unroll
+        for (int sub = 0; sub < SUBS; ++sub) {
+            const int c = b * NC + 32 * sub;
+            tmem_ld32(taddr + (uint32_t)c, v);
+            tmem_wait_ld();
+            tmem_regs_ready(v);
+            if (b == CW / NC - 1 && sub == SUBS - 1) release();
+            if (a.acc && t < a.M)
+                for (int j = 0; j < 32; ++j)
+                    if (n0 + c + j < a.N) {
+                        int x = 0;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x = i == j ? (int)v[i] : x;
+                        a.acc[(long long)t * a.ld_acc + n0 + c + j] = x;
+                    }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {   // eight columns: 32 bytes of FP32 or 16 bytes of a shorter type
+                float f[8];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint4 al = ld_shared16(consts + (uint32_t)(c + 8 * g + 4 * h) * 4u);
+                    uint4 bi = make_uint4(0u, 0u, 0u, 0u);
+                    if (has_bias) bi = ld_shared16(consts + (uint32_t)(CW + c + 8 * g + 4 * h) * 4u);
+                    const uint32_t aw[4] = {al.x, al.y, al.z, al.w}, bw[4] = {bi.x, bi.y, bi.z, bi.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        f[4 * h + i] = int8_value<SILU>((int)v[8 * g + 4 * h + i], sq, __uint_as_float(aw[i]), has_bias,
+                                                        __uint_as_float(bw[i]));
+                }
+                constexpr int PIECES = 8 * (int)sizeof(T) / 16;   // 16-byte pieces of these eight columns
+                uint32_t at[PIECES];
+#pragma unroll
+                for (int h = 0; h < PIECES; ++h) {
+                    const int piece = (sub * 32 + 8 * g) * (int)sizeof(T) / 16 + h;
+                    at[h] = stg + (uint32_t)lane * 128u + (uint32_t)((piece ^ (lane & 7)) << 4);
+                }
+                if (a.res) {
+                    float r[8];
+                    if (p.res_vec) {
+                        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint4 u = ld_shared16(at[h % PIECES]);
+                                r[4 * h] = __uint_as_float(u.x);
+                                r[4 * h + 1] = __uint_as_float(u.y);
+                                r[4 * h + 2] = __uint_as_float(u.z);
+                                r[4 * h + 3] = __uint_as_float(u.w);
+                            }
+                        } else {
+                            const uint4 u = ld_shared16(at[0]);
+                            const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float2 q = unpack2<T>(uw[i]);
+                                r[2 * i] = q.x;
+                                r[2 * i + 1] = q.y;
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int n = n0 + c + 8 * g + i;
+                            r[i] = t < a.M && n < a.N ? to_float(static_cast<const T *>(a.res)[(long long)t * a.ld_res + n]) : 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[i] = __fadd_rn(r[i], __fmul_rn(a.res_scale, f[i]));
+                }
+                if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        st_shared16(at[h % PIECES], __float_as_uint(f[4 * h]), __float_as_uint(f[4 * h + 1]),
+                                    __float_as_uint(f[4 * h + 2]), __float_as_uint(f[4 * h + 3]));
+                } else {
+                    st_shared16(at[0], pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+                }
+            }
+        }
+        if (p.tma_store) {
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) {
+                if (nb < a.N && row0 < a.M) tma_store_2d(ymap, stg, nb, row0);
+                bulk_commit_group();
+            }
+        } else {
+            __syncwarp();
+            int8_store_rows<T>(a, stg, row0, nb);
+            __syncwarp();
+        }
+    }
+}
+
+// float has no 16-bit packing; never called
+template <> KEA_DEVI uint32_t pack2<float>(float, float) { return 0u; }
+template <> KEA_DEVI float2 unpack2<float>(uint32_t) { return make_float2(0.f, 0.f); }
+
+template <typename T, bool SILU, int CTAS, int BN>
+__global__ void __launch_bounds__(Int8Tile<CTAS, BN>::THREADS, 1)
+int8_gemm_tile_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap wmap,
+                      const __grid_constant__ CUtensorMap ymap, const Int8TileArgs p) {
+    using Tile = Int8Tile<CTAS, BN>;
+    extern __shared__ uint8_t dyn_smem[];
+    __shared__ __align__(8) uint64_t bar_full[kI8MaxStages];    // (pairs: in the even CTA) both operands of a stage landed
+    __shared__ __align__(8) uint64_t bar_empty[kI8MaxStages];   // the MMAs are done with the stage
+    __shared__ __align__(8) uint64_t bar_acc_full[2];           // accumulator complete
+    __shared__ __align__(8) uint64_t bar_acc_empty[2];          // (pairs: in the even CTA) accumulator read by every epilogue warp
+    __shared__ __align__(8) uint64_t bar_drain;
+    __shared__ uint32_t tmem_slot;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = CTAS == 2 ? cluster_ctarank() : 0u;
+    const int worker = (int)blockIdx.x / CTAS, workers = (int)gridDim.x / CTAS;
+    const uint32_t base = (smem_u32(dyn_smem) + 1023u) & ~1023u;
+    const int S = p.stages;
+    const uint32_t A0 = base, B0 = base + (uint32_t)S * kI8Half;
+    const uint32_t STG0 = B0 + (uint32_t)S * Tile::B_BYTES, CONST0 = STG0 + Tile::STAGING;
+    constexpr uint32_t kCols = 2u * BN;   // two accumulators
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(smem_u32(&bar_full[s]), 1);
+            mbar_init(smem_u32(&bar_empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&bar_acc_full[b]), 1);
+            mbar_init(smem_u32(&bar_acc_empty[b]), CTAS * Tile::EPI_WARPS);
+        }
+        mbar_init(smem_u32(&bar_drain), 1);
+        fence_barrier_init();
+        prefetch_tensormap(&qmap);
+        prefetch_tensormap(&wmap);
+        prefetch_tensormap(&ymap);
+    }
+    if (warp == 1) {
+        if constexpr (CTAS == 2) {
+            tmem_alloc_pair(smem_u32(&tmem_slot), kCols);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(smem_u32(&tmem_slot), kCols);
+            tmem_relinquish();
+        }
+    }
+    tc_fence_before();
+    if constexpr (CTAS == 2) cluster_sync_all();
+    else __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    grid_dependency_wait();
+
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0, issued = 0;
+            uint32_t ph = 0;
+            for (int tile = worker; tile < p.tiles && ok; tile += workers) {
+                const int mt = tile / p.n_tiles, nt = tile - mt * p.n_tiles;
+                const int t0 = mt * 128 * CTAS + (int)rank * 128, n0 = nt * BN + (int)rank * (BN / CTAS);
+                for (int kb = 0; kb < p.kbs; ++kb) {
+                    if (issued >= S && !mbar_wait(smem_u32(&bar_empty[s]), ph ^ 1u, kOpWaitBudget)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t as = A0 + (uint32_t)s * kI8Half, bs = B0 + (uint32_t)s * Tile::B_BYTES;
+                    const uint32_t full = smem_u32(&bar_full[s]);
+                    if constexpr (CTAS == 2) {
+                        const uint32_t even = map_to_rank(full, 0u);
+                        if (rank == 0) mbar_arrive_expect_tx(full, 2u * Tile::STAGE);   // the bytes of both CTAs
+                        tma_load_2d_pair(as, &qmap, even, kb * kI8K, t0);
+                        tma_load_2d_pair(bs, &wmap, even, kb * kI8K, n0);
+                    } else {
+                        mbar_arrive_expect_tx(full, Tile::STAGE);
+                        tma_load_2d(as, &qmap, full, kb * kI8K, t0);
+                        tma_load_2d(bs, &wmap, full, kb * kI8K, n0);
+                    }
+                    if (issued < S) ++issued;
+                    if (++s == S) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+            // on failure the copies still in flight were issued before a wait that has lasted its whole bound (about 2 s)
+            if (!ok) report_error(p.a.err, KEA_DEVERR_TIMEOUT);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (rank == 0) {
+            const uint32_t idesc = idesc_i8(128u * CTAS, (uint32_t)BN);
+            const uint64_t ad0 = sw128_kmajor_desc(A0), bd0 = sw128_kmajor_desc(B0);
+            int j = 0, s = 0;
+            uint32_t ph = 0;
+            for (int tile = worker; tile < p.tiles; tile += workers, ++j) {
+                const int buf = j & 1;
+                const uint32_t use = (uint32_t)(j >> 1);
+                if (j >= 2) {
+                    const bool drained = CTAS == 2 ? mbar_wait_cluster(smem_u32(&bar_acc_empty[buf]), (use & 1u) ^ 1u, kOpWaitBudget)
+                                                   : mbar_wait(smem_u32(&bar_acc_empty[buf]), (use & 1u) ^ 1u, kOpWaitBudget);
+                    if (!__all_sync(0xFFFFFFFFu, drained)) {
+                        ok = false;
+                        break;
+                    }
+                }
+                tc_fence_after();
+                const uint32_t dcol = tmem + (uint32_t)buf * BN;
+                for (int kb = 0; kb < p.kbs; ++kb) {
+                    const bool ready = CTAS == 2 ? mbar_wait_cluster(smem_u32(&bar_full[s]), ph, kOpWaitBudget)
+                                                 : mbar_wait(smem_u32(&bar_full[s]), ph, kOpWaitBudget);
+                    if (!__all_sync(0xFFFFFFFFu, ready)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t ad = ad0 + (uint64_t)(((uint32_t)s * kI8Half) >> 4);
+                    const uint64_t bd = bd0 + (uint64_t)(((uint32_t)s * Tile::B_BYTES) >> 4);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = 0; kk < kI8K / 32; ++kk) {   // K = 32 per MMA: + 32 bytes = 2 descriptor units
+                            const uint32_t more = (kb > 0 || kk > 0) ? 1u : 0u;
+                            if constexpr (CTAS == 2) mma_i8_pair(dcol, ad + (uint64_t)(2 * kk), bd + (uint64_t)(2 * kk), idesc, more);
+                            else mma_i8(dcol, ad + (uint64_t)(2 * kk), bd + (uint64_t)(2 * kk), idesc, more);
+                        }
+                        if constexpr (CTAS == 2) mma_commit_pair(smem_u32(&bar_empty[s]), (uint16_t)3);
+                        else mma_commit(smem_u32(&bar_empty[s]));
+                    }
+                    __syncwarp();
+                    if (++s == S) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                if (elect_one()) {
+                    if constexpr (CTAS == 2) mma_commit_pair(smem_u32(&bar_acc_full[buf]), (uint16_t)3);
+                    else mma_commit(smem_u32(&bar_acc_full[buf]));
+                }
+                __syncwarp();
+            }
+            if (!ok && lane == 0) report_error(p.a.err, KEA_DEVERR_TIMEOUT);
+            // every MMA this warp issued completes before shared and tensor memory are given up
+            if (elect_one()) {
+                if constexpr (CTAS == 2) mma_commit_pair(smem_u32(&bar_drain), (uint16_t)1);
+                else mma_commit(smem_u32(&bar_drain));
+            }
+            __syncwarp();
+            mbar_wait(smem_u32(&bar_drain), 0u, kOpWaitBudget);
+            __syncwarp();
+        }
+    } else {
+        const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
+        const uint32_t stg = STG0 + (uint32_t)(ew * Tile::BUFS) * kI8Box;
+        const uint32_t consts = CONST0 + (uint32_t)(ew * Tile::CW) * 8u;
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * Tile::CW);
+        int j = 0, box = 0;
+        for (int tile = worker; tile < p.tiles; tile += workers, ++j) {
+            const int buf = j & 1;
+            const int mt = tile / p.n_tiles, nt = tile - mt * p.n_tiles;
+            const int row0 = mt * 128 * CTAS + (int)rank * 128 + quad * 32, n0 = nt * BN + half * Tile::CW;
+#pragma unroll
+            for (int i = 0; i < Tile::CW; i += 32) {   // this warp's channel constants, while the accumulator fills
+                const int n = n0 + i + lane;
+                const float al = n < p.a.N ? __ldg(p.a.alpha + n) : 0.f;
+                const float bi = p.a.bias && n < p.a.N ? __ldg(p.a.bias + n) : 0.f;
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(consts + (uint32_t)(i + lane) * 4u), "f"(al) : "memory");
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(consts + (uint32_t)(Tile::CW + i + lane) * 4u), "f"(bi) : "memory");
+            }
+            const float sq = row0 + lane < p.a.M ? p.a.qs[row0 + lane] : 0.f;
+            __syncwarp();
+            const bool done = mbar_wait_sleep(smem_u32(&bar_acc_full[buf]), (uint32_t)((j >> 1) & 1), kOpWaitBudget, 64);
+            if (!__all_sync(0xFFFFFFFFu, done)) {
+                if (lane == 0) report_error(p.a.err, KEA_DEVERR_TIMEOUT);
+                break;
+            }
+            tc_fence_after();
+            const uint32_t acc_empty = smem_u32(&bar_acc_empty[buf]);
+            int8_epilogue_tile<T, SILU, Tile::CW, Tile::BUFS>(p, &ymap, lanes + (uint32_t)(buf * BN), stg, consts, row0, n0, sq,
+                                                              box, [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CTAS == 2) mbar_arrive_cluster(map_to_rank(acc_empty, 0u));
+                    else mbar_arrive(acc_empty);
+                }
+            });
+        }
+        if (lane == 0) bulk_wait_group_read0();   // the staging space outlives the stores' reads of it
+        __syncwarp();
+    }
+
+    grid_launch_dependents();
+    tc_fence_before();
+    if constexpr (CTAS == 2) cluster_sync_relaxed_paths();
+    else __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        if constexpr (CTAS == 2) tmem_dealloc_pair(tmem, kCols);
+        else tmem_dealloc(tmem, kCols);
+    }
+}
+
+}  // namespace kea

@@ -41,6 +41,17 @@ template <> KEA_DEVI float2 unpack2<__nv_bfloat16>(uint32_t w) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
 
+constexpr long long kOpWaitBudget = 4000000000LL;   // SM clocks (about 2 s) before a wait gives up
+
+KEA_DEVI void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+KEA_DEVI uint4 ld_shared16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
 KEA_DEVI void report_error(uint32_t *word, uint32_t bits) { atomicOr(word, bits); }
 
 }  // namespace kea

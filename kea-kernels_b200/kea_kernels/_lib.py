@@ -33,7 +33,7 @@ EXPORTS = ("kea_lowbit_gemm", "kea_lowbit_gemm_noalloc", "kea_lowbit_choose_conf
            "kea_lowbit_int8_gemm", "kea_lowbit_residual_norm", "kea_lowbit_beam_select", "kea_lowbit_beam_reorder")
 CONV_PDL, CONV_QUANT_SILU = 1, 2
 INT8_SILU, INT8_PDL = 1, 2
-INT8_KERNEL_REG = 1
+INT8_KERNEL_REG, INT8_KERNEL_TILE64, INT8_KERNEL_TILE128, INT8_KERNEL_PAIR = 1, 2, 3, 4
 NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
 GATES = {"none": 0, "sigmoid": 1}   # KEA_GATE_*
 RNORM_PDL = BEAM_PDL = 1
