@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-import struct
 from pathlib import Path
 
 import torch
@@ -32,13 +31,7 @@ EXPORTS = ("kea_lowbit_gemm", "kea_lowbit_gemm_noalloc", "kea_lowbit_choose_conf
            "kea_lowbit_status_string", "kea_lowbit_version",
            "kea_lowbit_int8_gemm", "kea_lowbit_residual_norm", "kea_lowbit_beam_select", "kea_lowbit_beam_reorder")
 CONV_PDL, CONV_QUANT_SILU = 1, 2
-INT8_SILU, INT8_PDL = 1, 2
 INT8_KERNEL_REG, INT8_KERNEL_TILE64, INT8_KERNEL_TILE128, INT8_KERNEL_PAIR = 1, 2, 3, 4
-NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
-GATES = {"none": 0, "sigmoid": 1}   # KEA_GATE_*
-RNORM_PDL = BEAM_PDL = 1
-REORDER_MAX = 32
-TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # KEA_TYPE_*
 
 
 class GemmDesc(ctypes.Structure):
@@ -95,65 +88,6 @@ class AttentionDesc(ctypes.Structure):
                 ("scale", ctypes.c_float), ("flags", ctypes.c_int32)]
 
 
-class Int8Desc(ctypes.Structure):
-    _fields_ = [("q", ctypes.c_void_p), ("ldq", ctypes.c_int64), ("qs", ctypes.c_void_p), ("w", ctypes.c_void_p),
-                ("ldw", ctypes.c_int64), ("alpha", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("y", ctypes.c_void_p),
-                ("ldy", ctypes.c_int64), ("residual", ctypes.c_void_p), ("ld_residual", ctypes.c_int64),
-                ("acc", ctypes.c_void_p), ("ld_acc", ctypes.c_int64), ("residual_scale", ctypes.c_float),
-                ("m", ctypes.c_int32), ("n", ctypes.c_int32), ("k", ctypes.c_int32), ("y_type", ctypes.c_int32),
-                ("flags", ctypes.c_int32), ("kernel", ctypes.c_int32), ("error_word", ctypes.c_void_p)]
-
-
-class ResidualNormDesc(ctypes.Structure):
-    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("gate", ctypes.c_void_p),
-                ("ldx", ctypes.c_int64), ("ldy", ctypes.c_int64),
-                ("gate_clip_stride", ctypes.c_int64), ("gate_row_stride", ctypes.c_int64),
-                ("frames", ctypes.c_int32), ("gate_act", ctypes.c_int32), ("x_type", ctypes.c_int32),
-                ("y_type", ctypes.c_int32), ("h_type", ctypes.c_int32), ("post", ctypes.c_int32), ("pre", ctypes.c_int32),
-                ("scale", ctypes.c_float), ("post_eps", ctypes.c_float), ("pre_eps", ctypes.c_float),
-                ("post_weight", ctypes.c_void_p), ("post_bias", ctypes.c_void_p), ("pre_weight", ctypes.c_void_p),
-                ("pre_bias", ctypes.c_void_p), ("r", ctypes.c_void_p), ("h", ctypes.c_void_p), ("ldr", ctypes.c_int64),
-                ("ldh", ctypes.c_int64), ("q", ctypes.c_void_p), ("ldq", ctypes.c_int32), ("qs", ctypes.c_void_p),
-                ("m", ctypes.c_int32), ("d", ctypes.c_int32), ("flags", ctypes.c_int32)]
-
-
-class BeamDesc(ctypes.Structure):
-    _fields_ = [("logits", ctypes.c_void_p), ("ld_clip", ctypes.c_int64), ("ld_beam", ctypes.c_int64),
-                ("scores", ctypes.c_void_p), ("ended", ctypes.c_void_p), ("out_scores", ctypes.c_void_p),
-                ("parents", ctypes.c_void_p), ("labels", ctypes.c_void_p), ("out_ended", ctypes.c_void_p),
-                ("clips", ctypes.c_int32), ("beams", ctypes.c_int32), ("vocab", ctypes.c_int32),
-                ("width", ctypes.c_int32), ("end", ctypes.c_int32), ("logits_type", ctypes.c_int32),
-                ("flags", ctypes.c_int32)]
-
-
-class ReorderItem(ctypes.Structure):
-    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("src_group", ctypes.c_int64),
-                ("src_clip", ctypes.c_int64), ("src_beam", ctypes.c_int64), ("dst_group", ctypes.c_int64),
-                ("dst_clip", ctypes.c_int64), ("dst_beam", ctypes.c_int64), ("row_bytes", ctypes.c_int64),
-                ("groups", ctypes.c_int32)]
-
-
-class ReorderDesc(ctypes.Structure):
-    _fields_ = [("parents", ctypes.c_void_p), ("count", ctypes.c_int32),
-                ("clips", ctypes.c_int32), ("beams", ctypes.c_int32), ("width", ctypes.c_int32), ("flags", ctypes.c_int32),
-                ("error_word", ctypes.c_void_p)]
-
-
-_CODES = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f"}
-
-
-def packer(desc: type[ctypes.Structure]):
-    """A function from a descriptor's field values, in order (pointers as integers, 0 for none), to its bytes. Filling a
-    ctypes structure costs several microseconds of a call's host time, this a fraction of one."""
-    layout = struct.Struct("@" + "".join(_CODES[kind] for _, kind in desc._fields_) + "0P")
-    if layout.size != ctypes.sizeof(desc):
-        raise RuntimeError(f"{desc.__name__}: {layout.size} bytes, expected {ctypes.sizeof(desc)}")
-    return layout.pack
-
-
-pack_int8, pack_residual_norm = packer(Int8Desc), packer(ResidualNormDesc)
-pack_beam, pack_reorder, pack_reorder_item = packer(BeamDesc), packer(ReorderDesc), packer(ReorderItem)
-
 _lib = None
 
 
@@ -190,11 +124,9 @@ def lib() -> ctypes.CDLL:
         handle.kea_lowbit_glu_depthwise.restype = ctypes.c_int
         handle.kea_lowbit_rel_attention.argtypes = [ctypes.POINTER(AttentionDesc), ctypes.c_void_p]
         handle.kea_lowbit_rel_attention.restype = ctypes.c_int
-        for name in ("int8_gemm", "residual_norm", "beam_select"):   # descriptors come as packer()'s bytes
-            entry = getattr(handle, f"kea_lowbit_{name}")
-            entry.argtypes, entry.restype = [ctypes.c_char_p, ctypes.c_void_p], ctypes.c_int
-        handle.kea_lowbit_beam_reorder.argtypes = [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p]
-        handle.kea_lowbit_beam_reorder.restype = ctypes.c_int
+        for name, pointers in (("int8_gemm", 2), ("residual_norm", 2), ("beam_select", 2), ("beam_reorder", 3)):
+            entry = getattr(handle, f"kea_lowbit_{name}")   # called by _binding; argtypes for callers of the C ABI
+            entry.argtypes, entry.restype = [ctypes.c_void_p] * pointers, ctypes.c_int
         handle.kea_lowbit_read_error.argtypes = [ctypes.POINTER(ctypes.c_uint32)]
         handle.kea_lowbit_read_error.restype = ctypes.c_int
         handle.kea_lowbit_status_string.argtypes = [ctypes.c_int]
@@ -218,17 +150,25 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def call(entry: str, device: torch.device, *desc: bytes) -> None:
-    """kea_lowbit_<entry>(desc ..., stream) on `device` and its current stream; raises for a status that is not 0. The
-    current device is switched only where it is another one."""
-    function, index = getattr(_lib or lib(), entry), device.index
-    if index == torch._C._cuda_getDevice():
-        status = function(*desc, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(device):
-            status = function(*desc, torch._C._cuda_getCurrentRawStream(index))
-    if status != OK:
-        check(status, entry.removeprefix("kea_lowbit_"))
+_native = None
+
+
+def native():
+    """The C++ entry points of lowbit's 8-bit linear map, residual-norm step and beam search (csrc/binding.cpp), bound to
+    the loaded library; raises RuntimeError when the extension is missing."""
+    global _native
+    if _native is None:
+        handle = lib()
+        try:
+            from kea_kernels import _binding
+        except ImportError as e:
+            raise RuntimeError("kea_kernels/_binding.so is missing or does not load: build it with "
+                               f"`python kea-kernels_b200/build.py` ({e})") from e
+        names = ("int8_gemm", "residual_norm", "beam_select", "beam_reorder", "status_string")
+        _binding.bind(*(ctypes.cast(getattr(handle, f"kea_lowbit_{name}"), ctypes.c_void_p).value for name in names),
+                      torch.nn.LayerNorm, torch.nn.RMSNorm)
+        _native = _binding
+    return _native
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

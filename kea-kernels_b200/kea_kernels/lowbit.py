@@ -16,7 +16,7 @@ import math
 from typing import NamedTuple, Sequence
 
 import torch
-from torch import Tensor, nn
+from torch import Tensor
 
 from kea_kernels import _lib
 
@@ -357,153 +357,8 @@ def int8_linear(q: Tensor, qs: Tensor, weight: Tensor, alpha: Tensor, bias: Tens
     FP16 or BF16), or `out` (unit column stride) where given. residual: [m, n] of the output's type, unit column stride; may
     be `out` itself. Rows of q and weight are 16-byte aligned; with `k`, columns >= k of both are ignored. acc (INT32
     [m, n], unit column stride) receives the sums. kernel forces one of INT8_KERNEL_* (0: chosen by the shape)."""
-    _require_cuda(q, "q")
-    device = q.device
-    if q.dtype is not torch.int8 or weight.dtype is not torch.int8 or q.dim() != 2 or weight.dim() != 2:
-        raise ValueError("q and weight must be int8 [m, k] and [n, k]")
-    (m, qk), (n, wk) = q.shape, weight.shape
-    if k is None:
-        k = wk
-        if qk != k:
-            raise ValueError(f"q has {qk} columns and weight {k}")
-    elif not 1 <= k <= min(qk, wk):
-        raise ValueError(f"k must lie between 1 and the columns of q and weight, got {k}")
-    ldq, ldw = _matrix(q, "q", device), _matrix(weight, "weight", device)
-    ldq, ldw = ldq if m > 1 else _round_up(k, 16), ldw if n > 1 else _round_up(k, 16)
-    _vector(qs, m, "qs", device)
-    _vector(alpha, n, "alpha", device)
-    if bias is not None:
-        _vector(bias, n, "bias", device)
-    if out is None:
-        out, ldy = torch.empty((m, n), device=device, dtype=dtype), n
-    else:
-        dtype, ldy = out.dtype, _matrix(out, "out", device, (m, n))
-    kind = _lib.TYPES.get(dtype)
-    if kind is None:
-        raise ValueError(f"the output must be FP32, FP16 or BF16, got {dtype}")
-    res = ld_res = sums = ld_sums = 0
-    if residual is not None:
-        if residual.dtype is not dtype:
-            raise ValueError(f"residual must have the output's type {dtype}")
-        res, ld_res = residual.data_ptr(), _matrix(residual, "residual", device, (m, n))
-    if acc is not None:
-        if acc.dtype is not torch.int32:
-            raise ValueError("acc must be int32")
-        sums, ld_sums = acc.data_ptr(), _matrix(acc, "acc", device, (m, n))
-    if m == 0 or n == 0:
-        return out
-    _lib.call("kea_lowbit_int8_gemm", device, _lib.pack_int8(
-        q.data_ptr(), ldq, qs.data_ptr(), weight.data_ptr(), ldw, alpha.data_ptr(),
-        0 if bias is None else bias.data_ptr(), out.data_ptr(), ldy, res, ld_res, sums, ld_sums, residual_scale, m, n, k, kind,
-        (_lib.INT8_SILU if silu else 0) | (_lib.INT8_PDL if pdl else 0), kernel, _word(error_word, device)))
-    return out
-
-
-def _matrix(t: Tensor, name: str, device: torch.device, shape: tuple[int, int] | None = None) -> int:
-    """The row stride of a matrix of unit column stride on `device` (a single row's stride says nothing: its width)."""
-    rows, cols = t.shape if shape is None else shape
-    if shape is not None and t.shape != shape:
-        raise ValueError(f"{name} must be [{rows}, {cols}], got {list(t.shape)}")
-    stride = t.stride()
-    if stride[1] != 1 and cols > 1:
-        raise ValueError(f"{name} must have unit column stride")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}")
-    return stride[0] if rows > 1 else cols
-
-
-def _vector(t: Tensor, n: int, name: str, device: torch.device) -> None:
-    if t.dtype is not torch.float32 or t.shape != (n,) or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} must be contiguous FP32 [{n}] on {device}")
-
-
-def _word(error_word: Tensor | None, device: torch.device) -> int:
-    if error_word is None:
-        return 0
-    if error_word.dtype is not torch.int32 or error_word.numel() != 1 or error_word.device != device:
-        raise ValueError(f"error_word must be one int32 on {device}")
-    return error_word.data_ptr()
-
-
-def _norm_args(norm, d: int, device: torch.device, what: str) -> tuple[int, float, int, int]:
-    """(kind, eps, weight pointer, bias pointer) of an nn.LayerNorm or nn.RMSNorm over the last dimension, or of None."""
-    if norm is None:
-        return _lib.NORM_NONE, 0.0, 0, 0
-    parameters = norm._parameters if isinstance(norm, nn.Module) else {}
-    if isinstance(norm, nn.LayerNorm):
-        kind, bias = _lib.NORM_LAYER, parameters["bias"]
-    elif isinstance(norm, nn.RMSNorm):
-        kind, bias = _lib.NORM_RMS, None
-    else:
-        raise ValueError(f"{what} must be an nn.LayerNorm or an nn.RMSNorm")
-    weight = parameters["weight"]
-    if weight is None:
-        raise ValueError(f"{what} needs a weight")
-    _vector(weight, d, f"{what}.weight", device)
-    if bias is not None:
-        _vector(bias, d, f"{what}.bias", device)
-    eps = torch.finfo(torch.float32).eps if norm.eps is None else norm.eps
-    return kind, eps, weight.data_ptr(), 0 if bias is None else bias.data_ptr()
-
-
-def _rows(t: Tensor, name: str) -> int:
-    """The one stride at which the rows of t [..., D] lie."""
-    d = t.shape[-1]
-    if t.is_contiguous():
-        return d
-    if t.stride(-1) != 1 and d > 1:
-        raise ValueError(f"{name} must have unit stride along its last dimension")
-    rows, step = 1, 0
-    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
-        if size == 1:
-            continue
-        if rows == 1:
-            step = stride
-        elif stride != step * rows:
-            raise ValueError(f"{name}'s rows must lie at one stride")
-        rows *= size
-    return step if rows > 1 else d
-
-
-def _residual_norm(x: Tensor, y: Tensor, h: Tensor | None, q: Tensor | None, qs: Tensor | None, out: Tensor | None,
-                   post_norm, gate, gate_act, scale, pre_norm, pdl) -> Tensor:
-    device, shape, types = x.device, x.shape, _lib.TYPES
-    if x.dim() < 2 or y.shape != shape or x.dtype not in types or y.dtype not in types:
-        raise ValueError("x and y must be FP32, FP16 or BF16 tensors [..., T, D] of one shape")
-    d, frames = shape[-1], shape[-2]
-    if out is None:
-        out = torch.empty(shape, device=device, dtype=x.dtype)
-    elif out.shape != shape or out.dtype is not x.dtype or out.device != device:
-        raise ValueError(f"out must have x's shape and type on {device}")
-    if y.device != device:
-        raise ValueError(f"y must be on {device}")
-    act = _lib.GATES.get(gate_act)
-    if act is None:
-        raise ValueError(f"gate_act must be one of {tuple(_lib.GATES)}, got {gate_act!r}")
-    gates = gate_clip = gate_row = 0
-    if gate is not None:
-        if gate.dtype is not y.dtype or gate.device != device or gate.shape[-1:] != (d,) or (gate.stride(-1) != 1 and d > 1):
-            raise ValueError(f"gate must be [..., {d}] of y's type on {device} with unit stride along its last dimension")
-        if gate.shape == shape:
-            gate_row = _rows(gate, "gate")
-            gate_clip = frames * gate_row
-        elif gate.dim() == 2 and len(shape) == 3 and gate.shape[0] == shape[0]:
-            gate_clip = gate.stride(0)
-        elif gate.dim() != 1:
-            raise ValueError(f"gate must be [{d}], one row per clip [B, {d}] of x [B, T, {d}], or of x's shape")
-        gates = gate.data_ptr()
-    post, post_eps, post_weight, post_bias = _norm_args(post_norm, d, device, "post_norm")
-    pre, pre_eps, pre_weight, pre_bias = _norm_args(pre_norm, d, device, "pre_norm")
-    m = x.numel() // d if d else 0
-    if m == 0:
-        return out
-    _lib.call("kea_lowbit_residual_norm", device, _lib.pack_residual_norm(
-        x.data_ptr(), y.data_ptr(), gates, _rows(x, "x"), _rows(y, "y"), gate_clip, gate_row, frames, act,
-        types[x.dtype], types[y.dtype], 0 if h is None else types[h.dtype], post, pre, scale, post_eps, pre_eps,
-        post_weight, post_bias, pre_weight, pre_bias, out.data_ptr(), 0 if h is None else h.data_ptr(), _rows(out, "out"), d,
-        0 if q is None else q.data_ptr(), 0 if q is None else q.stride(0), 0 if qs is None else qs.data_ptr(), m, d,
-        _lib.RNORM_PDL if pdl else 0))
-    return out
+    return (_lib._native or _lib.native()).int8_linear(q, qs, weight, alpha, bias, out, k, dtype, silu, residual,
+                                                       residual_scale, acc, kernel, pdl, error_word)
 
 
 def residual_norm(x: Tensor, y: Tensor, *, post_norm=None, gate: Tensor | None = None, gate_act: str = "none",
@@ -515,12 +370,7 @@ def residual_norm(x: Tensor, y: Tensor, *, post_norm=None, gate: Tensor | None =
     x [B, T, D], or of x's shape, taken as it is or through the logistic function (gate_act "sigmoid"). r has x's type
     (written to `out` where given, x itself included) and h `dtype` (y's by default). h is the norm of r before its
     rounding; all arithmetic is FP32."""
-    _require_cuda(x, "x")
-    dtype = y.dtype if dtype is None else dtype
-    if dtype not in _lib.TYPES:
-        raise ValueError(f"h must be FP32, FP16 or BF16, got {dtype}")
-    h = torch.empty(x.shape, device=x.device, dtype=dtype)
-    return _residual_norm(x, y, h, None, None, out, post_norm, gate, gate_act, scale, pre_norm, pdl), h
+    return (_lib._native or _lib.native()).residual_norm(x, y, post_norm, gate, gate_act, scale, pre_norm, out, pdl, dtype)
 
 
 def residual_norm_quantized(x: Tensor, y: Tensor, *, post_norm=None, gate: Tensor | None = None, gate_act: str = "none",
@@ -528,13 +378,8 @@ def residual_norm_quantized(x: Tensor, y: Tensor, *, post_norm=None, gate: Tenso
                             pdl: bool = False) -> tuple[Tensor, Tensor, Tensor]:
     """residual_norm with the next 8-bit projection's quantizer in the same pass -> (r, q, qs): q INT8 [m, D] codes of h's
     rows (held 16-byte aligned) with one FP32 scale each, qs [m], as quantize() forms one part. h is never written."""
-    _require_cuda(x, "x")
-    d = x.shape[-1]
-    m = x.numel() // max(1, d)
-    q = torch.empty((m, _round_up(d, 16)), device=x.device, dtype=torch.int8)
-    qs = torch.empty(m, device=x.device, dtype=torch.float32)
-    r = _residual_norm(x, y, None, q, qs, out, post_norm, gate, gate_act, scale, pre_norm, pdl)
-    return r, q if q.shape[1] == d else q[:, :d], qs
+    return (_lib._native or _lib.native()).residual_norm_quantized(x, y, post_norm, gate, gate_act, scale, pre_norm, out,
+                                                                   pdl)
 
 
 class BeamStep(NamedTuple):
@@ -555,44 +400,8 @@ def beam_select(logits: Tensor, scores: Tensor, width: int | None = None, *, end
     come by (hypothesis, label). Logits of -inf and those that are not numbers are masked; a hypothesis with an infinite
     score or log-sum offers nothing; places that nothing fills take what is not offered by (hypothesis, label), with score
     -inf. At most 32 hypotheses and places. `out`: tensors to write to (rows of a history, for instance)."""
-    _require_cuda(logits, "logits")
-    shape, strides, kind = logits.shape, logits.stride(), _lib.TYPES.get(logits.dtype)
-    if len(shape) != 3 or kind is None or (strides[2] != 1 and shape[2] > 1):
-        raise ValueError("logits must be FP32, FP16 or BF16 [clips, beams, vocab] with unit stride along the labels")
-    clips, beams, vocab = shape
-    device, given, width = logits.device, (clips, beams), beams if width is None else width
-    if scores.dtype is not torch.float32 or scores.shape != given or scores.device != device or not scores.is_contiguous():
-        raise ValueError(f"scores must be contiguous FP32 [{clips}, {beams}] on {device}")
-    if end is not None and not 0 <= end < vocab:
-        raise ValueError(f"end must be a label below {vocab}, got {end}")
-    if ended is not None:
-        if end is None:
-            raise ValueError("ended hypotheses need the label `end`")
-        if ended.dtype not in (torch.bool, torch.uint8) or ended.shape != given or ended.device != device \
-                or not ended.is_contiguous():
-            raise ValueError(f"ended must be contiguous bool [{clips}, {beams}] on {device}")
-    if width < 1 or width > beams * vocab:
-        raise ValueError(f"width must lie between 1 and beams * vocab, got {width}")
-    if out is None:
-        place = (clips, width)
-        out = BeamStep(torch.empty(place, device=device), torch.empty(place, device=device, dtype=torch.int32),
-                       torch.empty(place, device=device, dtype=torch.int32),
-                       None if end is None else torch.empty(place, device=device, dtype=torch.bool))
-    else:
-        for t, name, types in ((out.scores, "scores", (torch.float32,)), (out.parents, "parents", (torch.int32,)),
-                               (out.tokens, "tokens", (torch.int32,)), (out.ended, "ended", (torch.bool, torch.uint8))):
-            if t is None and name == "ended":
-                continue
-            if t.dtype not in types or t.shape != (clips, width) or t.device != device or not t.is_contiguous():
-                raise ValueError(f"out.{name} must be contiguous {types[0]} [{clips}, {width}] on {device}")
-    if clips == 0:
-        return out
-    _lib.call("kea_lowbit_beam_select", device, _lib.pack_beam(
-        logits.data_ptr(), strides[0], strides[1], scores.data_ptr(), 0 if ended is None else ended.data_ptr(),
-        out.scores.data_ptr(), out.parents.data_ptr(), out.tokens.data_ptr(),
-        0 if out.ended is None else out.ended.data_ptr(), clips, beams, vocab, width, -1 if end is None else end, kind,
-        _lib.BEAM_PDL if pdl else 0))
-    return out
+    step = (_lib._native or _lib.native()).beam_select(logits, scores, width, end, ended, out, pdl)
+    return BeamStep._make(step) if out is None else out
 
 
 def beam_reorder(states: Sequence[Tensor], parents: Tensor, *, batch_dim: int = 0, out: Sequence[Tensor] | None = None,
@@ -602,60 +411,4 @@ def beam_reorder(states: Sequence[Tensor], parents: Tensor, *, batch_dim: int = 
     result[..., b, w, ...] = state[..., b, parents[b, w], ...], all states in one launch. parents int32 [clips, width].
     `out`: tensors to write to, not the states themselves. A parent outside the hypotheses leaves zeros and sets
     DEVERR_INDEX in the error word."""
-    _require_cuda(parents, "parents")
-    if parents.dtype is not torch.int32 or parents.dim() != 2 or not parents.is_contiguous():
-        raise ValueError("parents must be contiguous int32 [clips, width]")
-    if out is not None and len(out) != len(states):
-        raise ValueError("one output per state")
-    device, chosen = parents.device, parents.shape
-    clips, width = chosen
-    results, items, beams = [], [], None
-    for i, s in enumerate(states):
-        shape = s.shape
-        if len(shape) < batch_dim + 2 or shape[batch_dim] != clips or s.device != device:
-            raise ValueError(f"state {i} must have {clips} clips at dimension {batch_dim} on {device}")
-        if beams is None:
-            beams = shape[batch_dim + 1]
-        elif shape[batch_dim + 1] != beams:
-            raise ValueError("every state must have the same number of hypotheses")
-        want = shape if width == beams else shape[:batch_dim + 1] + (width,) + shape[batch_dim + 2:]
-        if out is None:
-            r = torch.empty(want, device=device, dtype=s.dtype)
-        else:
-            r = out[i]
-            if r.shape != want or r.dtype is not s.dtype or r.device != device:
-                raise ValueError(f"output {i} must be {s.dtype} {tuple(want)} on {device}")
-            if r.data_ptr() == s.data_ptr() and r.numel():
-                raise ValueError(f"output {i} may not be the state itself")
-        results.append(r)
-        if r.numel() == 0:
-            continue
-        src, group, clip, beam, row, groups = _state_layout(s, batch_dim, "state", i)
-        dst, to_group, to_clip, to_beam, _, _ = _state_layout(r, batch_dim, "output", i)
-        items.append(_lib.pack_reorder_item(src, dst, group, clip, beam, to_group, to_clip, to_beam, row, groups))
-    word = _word(error_word, device)
-    for first in range(0, len(items), _lib.REORDER_MAX):
-        part = items[first:first + _lib.REORDER_MAX]
-        _lib.call("kea_lowbit_beam_reorder", device, _lib.pack_reorder(
-            parents.data_ptr(), len(part), clips, beams, width, _lib.BEAM_PDL if pdl else 0, word), b"".join(part))
-    return results
-
-
-def _state_layout(t: Tensor, batch_dim: int, name: str, index: int) -> tuple[int, int, int, int, int, int]:
-    """(pointer, byte strides of group, clip and hypothesis, bytes of a row, groups) of a beam search's state."""
-    shape, stride, size = t.shape, t.stride(), t.element_size()
-    row = 1
-    for i in range(len(shape) - 1, batch_dim + 1, -1):
-        if shape[i] > 1 and stride[i] != row:
-            raise ValueError(f"{name} {index}: what follows the hypotheses must be contiguous")
-        row *= shape[i]
-    groups, group = 1, 0
-    for i in range(batch_dim - 1, -1, -1):
-        if shape[i] == 1:
-            continue
-        if groups == 1:
-            group = stride[i]
-        elif stride[i] != group * groups:
-            raise ValueError(f"{name} {index}: the dimensions before the clips must lie at one stride")
-        groups *= shape[i]
-    return t.data_ptr(), group * size, stride[batch_dim] * size, stride[batch_dim + 1] * size, row * size, groups
+    return (_lib._native or _lib.native()).beam_reorder(states, parents, batch_dim, out, pdl, error_word)
