@@ -27,32 +27,25 @@ struct Int8Args {
     uint32_t *err;
 };
 
-// y / (1 + 2^(-y log2 e)) with the hardware's approximate exponential and division (2 units in the last place each; a
-// denominator above 2^126 gives 0).
-KEA_DEVI float int8_silu(float y) {
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(y, -1.4426950408889634f)));
-    return __fdividef(y, __fadd_rn(1.0f, e));
-}
+// The bias where there is none: r * alpha + -0 is r * alpha, its sign included.
+constexpr float kI8NoBias = -0.0f;
 
-// RN(a) without the conversion instruction, whose pipe is a quarter as wide as the SiLU's exponential and reciprocal
-// leave free: with a = 65536 h + l, the float of bits 0x4B000000 | (h + 2^15) is 2^23 + 2^15 + h and that of 0x4B000000 | l
-// is 2^23 + l; the fma is exact (a multiple of 65536 below 2^40), the addition rounds once.
-KEA_DEVI float int_to_float(int a) {
-    const float h = __uint_as_float(__byte_perm((uint32_t)a ^ 0x80000000u, 0x4B000000u, 0x7632));
-    const float l = __uint_as_float(__byte_perm((uint32_t)a, 0x4B000000u, 0x7610));
-    return __fadd_rn(__fmaf_rn(h, 65536.0f, -551911686144.0f), l);   // 65536 (2^23 + 2^15 + 128)
-}
-
-// One output before the skip connection.
+// Two outputs before the skip connection. SiLU: y / (1 + 2^(-y log2 e)) with the hardware's approximate exponential and
+// reciprocal (2 and 1 units in the last place; a denominator above 2^126 gives 0).
 template <bool SILU>
-KEA_DEVI float int8_value(int acc, float s, float alpha, bool has_bias, float bias) {
-    const float r = __fmul_rn(SILU ? int_to_float(acc) : __int2float_rn(acc), s);
-    const float v = has_bias ? __fmaf_rn(r, alpha, bias) : __fmul_rn(r, alpha);
-    return SILU ? int8_silu(v) : v;
-}
-KEA_DEVI float int8_value(int acc, float s, float alpha, bool has_bias, float bias, bool silu) {
-    return silu ? int8_value<true>(acc, s, alpha, has_bias, bias) : int8_value<false>(acc, s, alpha, has_bias, bias);
+KEA_DEVI uint64_t int8_values(int a0, int a1, uint64_t s, uint64_t alpha, uint64_t bias) {
+    uint64_t y = fma2(mul2(pair_of(__int2float_rn(a0), __int2float_rn(a1)), s), alpha, bias);
+    if constexpr (SILU) {
+        float t0, t1;
+        unpair(mul2(y, pair_of(-1.4426950408889634f, -1.4426950408889634f)), t0, t1);
+        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t0));
+        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t1));
+        unpair(add2(pair_of(t0, t1), pair_of(1.0f, 1.0f)), t0, t1);
+        asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(t0));
+        asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(t1));
+        y = mul2(y, pair_of(t0, t1));
+    }
+    return y;
 }
 
 template <typename T>

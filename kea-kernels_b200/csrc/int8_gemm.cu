@@ -147,7 +147,9 @@ cudaError_t launch_tile_as(const kea_host::Device &dev, const kea::Int8Args &a, 
     p.tma_store = map_output(dev, &ymap, a) ? 1 : 0;
     p.res_vec = a.res && aligned(a.res, 16) && (a.ld_res * (long long)size) % 16 == 0 && ((size_t)a.N * size) % 16 == 0;
     const Launch l(dim3((unsigned)(workers * CTAS), 1, 1), Tile::THREADS, Tile::smem(p.stages), stream, pdl, CTAS);
-    return cudaLaunchKernelEx(&l.cfg, kea::int8_gemm_tile_kernel<T, SILU, CTAS, BN>, qmap, wmap, ymap, p);
+    if (a.acc || (a.res && !p.res_vec))
+        return cudaLaunchKernelEx(&l.cfg, kea::int8_gemm_tile_kernel<T, SILU, true, CTAS, BN>, qmap, wmap, ymap, p);
+    return cudaLaunchKernelEx(&l.cfg, kea::int8_gemm_tile_kernel<T, SILU, false, CTAS, BN>, qmap, wmap, ymap, p);
 }
 
 template <typename T>
@@ -170,23 +172,24 @@ int choose(const kea::Int8Args &a, int sms) {
     return KEA_INT8_KERNEL_TILE64;
 }
 
-template <typename T, bool SILU>
+template <typename T, bool SILU, bool EXTRA>
 bool attributes() {
     const auto set = [](const void *kernel) {
         return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynSmem) == cudaSuccess;
     };
-    return set((const void *)kea::int8_gemm_tile_kernel<T, SILU, 1, 64>) &&
-           set((const void *)kea::int8_gemm_tile_kernel<T, SILU, 1, 128>) &&
-           set((const void *)kea::int8_gemm_tile_kernel<T, SILU, 2, 256>);
+    return set((const void *)kea::int8_gemm_tile_kernel<T, SILU, EXTRA, 1, 64>) &&
+           set((const void *)kea::int8_gemm_tile_kernel<T, SILU, EXTRA, 1, 128>) &&
+           set((const void *)kea::int8_gemm_tile_kernel<T, SILU, EXTRA, 2, 256>);
+}
+template <typename T>
+bool attributes() {
+    return attributes<T, false, false>() && attributes<T, false, true>() && attributes<T, true, false>() && attributes<T, true, true>();
 }
 
 }  // namespace
 
 int kea_host::setup_int8_gemm() {
-    return attributes<float, false>() && attributes<float, true>() && attributes<__half, false>() && attributes<__half, true>() &&
-                   attributes<__nv_bfloat16, false>() && attributes<__nv_bfloat16, true>()
-               ? KEA_OK
-               : KEA_ERR_CUDA;
+    return attributes<float>() && attributes<__half>() && attributes<__nv_bfloat16>() ? KEA_OK : KEA_ERR_CUDA;
 }
 
 extern "C" int kea_lowbit_int8_gemm(const KeaInt8Desc *d, void *stream) {

@@ -129,15 +129,17 @@ __global__ void __launch_bounds__(kI8RegThreads, 2) int8_gemm_reg_kernel(const I
             part[(row + 1) * ld + ch + 8] = acc[c][r][3];
         }
     __syncthreads();
-    const bool has_bias = a.bias != nullptr;
     for (int i = threadIdx.x; i < R * CN; i += kI8RegThreads) {
         const int row = i / CN, ch = i - row * CN, m = m0 + row, n = c0 + ch;
         if (m >= a.M || n >= a.N) continue;
         int v = 0;
         for (int w = 0; w < KS; ++w) v += rsm[(w * R + row) * ld + ch];
         if (a.acc) a.acc[(long long)m * a.ld_acc + n] = v;
-        int8_store<T>(a, m, n, int8_value(v, a.qs[m], __ldg(a.alpha + n), has_bias, has_bias ? __ldg(a.bias + n) : 0.f,
-                                          a.silu != 0));
+        const uint64_t s = pair_of(a.qs[m], 0.f), alpha = pair_of(__ldg(a.alpha + n), 0.f);
+        const uint64_t bias = pair_of(a.bias ? __ldg(a.bias + n) : kI8NoBias, 0.f);
+        float y, unused;
+        unpair(a.silu ? int8_values<true>(v, 0, s, alpha, bias) : int8_values<false>(v, 0, s, alpha, bias), y, unused);
+        int8_store<T>(a, m, n, y);
     }
 }
 

@@ -8,7 +8,7 @@
 // epilogue of one tile runs while the MMAs of the next fill the other.
 //
 // Warps: 0 producer (one lane: TMA loads); 1 tensor memory and MMA issue; 2 .. epilogue, warp pair (w % 4) reading the
-// 32 tensor-memory lanes it may, in HALVES column halves: TMEM -> scales, bias, SiLU, skip connection -> boxes of 32 rows
+// 32 tensor-memory lanes it may and 64 columns: TMEM -> scales, bias, SiLU, skip connection -> boxes of 32 rows
 // x 128 bytes staged in shared memory (128-byte swizzle) -> TMA stores, or row-wise stores where the output's rows are
 // not 16-byte aligned. Every wait is bounded; one that runs out is reported in the error word and the kernel ends.
 #pragma once
@@ -24,9 +24,9 @@ constexpr int kI8MaxStages = 8;
 
 template <int CTAS, int BN>
 struct Int8Tile {
-    static constexpr int HALVES = BN >= 128 ? 2 : 1, EPI_WARPS = 4 * HALVES, THREADS = 64 + 32 * EPI_WARPS;
-    static constexpr int CW = BN / HALVES;                                // columns per epilogue warp
-    static constexpr int BUFS = 2;                                        // staging boxes per epilogue warp
+    static constexpr int CW = BN == 256 ? 128 : 64;                       // columns per epilogue warp
+    static constexpr int EPI_WARPS = 4 * (BN / CW), THREADS = 64 + 32 * EPI_WARPS;
+    static constexpr int BUFS = BN == 256 ? 1 : 2;                         // staging boxes per epilogue warp
     static constexpr uint32_t B_BYTES = (uint32_t)(BN / CTAS) * kI8K, STAGE = kI8Half + B_BYTES;
     static constexpr uint32_t STAGING = EPI_WARPS * BUFS * kI8Box, CONSTS = EPI_WARPS * CW * 8u;
     static constexpr uint32_t smem(int stages) { return 1024u + (uint32_t)stages * STAGE + STAGING + CONSTS; }
@@ -50,19 +50,25 @@ KEA_DEVI void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
     tmem_ld16(taddr + 16u, *reinterpret_cast<uint32_t(*)[16]>(&v[16]));
 }
 
-// The skip connection's 32 rows x 128 bytes in front of a box, read row-wise into the staging space (swizzled).
+// The skip connection's 32 rows x 128 bytes in front of a box: row-wise loads into registers (ahead of their use), then
+// into the staging space (swizzled).
 template <typename T>
-KEA_DEVI void int8_stage_residual(const Int8Args &a, uint32_t stg, int row0, int n0) {
-    const int lane = threadIdx.x & 31, piece = lane & 7;
-    constexpr int E = 16 / sizeof(T);
-    const int n = n0 + piece * E;
+KEA_DEVI void int8_load_residual(const Int8Args &a, uint4 (&v)[8], int row0, int n0) {
+    const int lane = threadIdx.x & 31, n = n0 + (lane & 7) * (16 / (int)sizeof(T));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int r = 4 * i + (lane >> 3), t = row0 + r;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        const int t = row0 + 4 * i + (lane >> 3);
+        v[i] = make_uint4(0u, 0u, 0u, 0u);
         if (t < a.M && n < a.N)
-            v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.res) + (long long)t * a.ld_res + n);
-        st_shared16(stg + (uint32_t)r * 128u + (uint32_t)((piece ^ (r & 7)) << 4), v.x, v.y, v.z, v.w);
+            v[i] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.res) + (long long)t * a.ld_res + n);
+    }
+}
+KEA_DEVI void int8_stage_residual(const uint4 (&v)[8], uint32_t stg) {
+    const int lane = threadIdx.x & 31, piece = lane & 7;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        st_shared16(stg + (uint32_t)r * 128u + (uint32_t)((piece ^ (r & 7)) << 4), v[i].x, v[i].y, v[i].z, v[i].w);
     }
 }
 
@@ -70,7 +76,9 @@ KEA_DEVI void int8_stage_residual(const Int8Args &a, uint32_t stg, int row0, int
 template <typename T>
 KEA_DEVI void int8_store_rows(const Int8Args &a, uint32_t stg, int row0, int n0) {
     const int lane = threadIdx.x & 31;
-    for (int r = 0; r < 32 && row0 + r < a.M; ++r) {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+        if (row0 + r >= a.M) break;
         uint32_t w;
         asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(stg + (uint32_t)r * 128u + (uint32_t)(((lane >> 2) ^ (r & 7)) << 4) + (uint32_t)(lane & 3) * 4u) : "memory");
         T *dst = static_cast<T *>(a.y) + (long long)(row0 + r) * a.ldy;
@@ -84,117 +92,113 @@ KEA_DEVI void int8_store_rows(const Int8Args &a, uint32_t stg, int row0, int n0)
     }
 }
 
-// One epilogue warp's 32 rows x CW columns of a finished tile. `release` hands the accumulator back.
-template <typename T, bool SILU, int CW, int BUFS, typename Release>
+// One epilogue warp's 32 rows x CW columns of a finished tile, 32 columns at a time. The loop is not unrolled: its body is
+// some 600 instructions that eight warps run at different places, and four copies of it missed the instruction cache (the
+// largest stall of the kernel, 128 x 256 outputs per SM 7 us instead of 3). `ahead` holds the first box's skip connection
+// (res_vec), `release` hands the accumulator back. EXTRA: the sums are wanted too, or the skip connection's rows are not
+// 16-byte aligned.
+template <typename T, bool SILU, bool EXTRA, int CW, int BUFS, typename Release>
 KEA_DEVI void int8_epilogue_tile(const Int8TileArgs &p, const CUtensorMap *ymap, uint32_t taddr, uint32_t stg0, uint32_t consts,
-                                 int row0, int n0, float sq, int &box, Release release) {
+                                 int row0, int n0, uint64_t sq, int &box, uint4 (&ahead)[8], Release release) {
     const Int8Args &a = p.a;
     const int lane = threadIdx.x & 31, t = row0 + lane;
-    constexpr int NC = 128 / (int)sizeof(T), SUBS = NC / 32;
-    const bool has_bias = a.bias != nullptr;
-    uint32_t v[32];
+    constexpr int NC = 128 / (int)sizeof(T), CHUNKS = CW / 32, PER = NC / 32;   // columns per box, chunks, chunks per box
+    constexpr int PIECES = 32 * (int)sizeof(T) / 16, E = 16 / (int)sizeof(T);   // 16-byte pieces of a chunk, values in one
+    const bool has_res = a.res != nullptr, staged = has_res && (!EXTRA || p.res_vec);
 #pragma unroll 1
-    for (int b = 0; b < CW / NC; ++b, ++box) {
-        const uint32_t stg = stg0 + (uint32_t)(box % BUFS) * kI8Box;
-        if (lane == 0) {   // the store that last read this space is done with it
-            if constexpr (BUFS == 2) bulk_wait_group_read1();
-            else bulk_wait_group_read0();
-        }
-        __syncwarp();
-        const int nb = n0 + b * NC;
-        if (a.res && p.res_vec) {
-            int8_stage_residual<T>(a, stg, row0, nb);
+    for (int i = 0; i < CHUNKS; ++i) {
+        const uint32_t stg = stg0 + (uint32_t)(box % BUFS) * kI8Box, rowaddr = stg + (uint32_t)lane * 128u;
+        const int c = 32 * i, nb = n0 + i / PER * NC, piece0 = i % PER * PIECES;
+        uint32_t v[32];
+        tmem_ld32(taddr + (uint32_t)c, v);
+        if (i % PER == 0) {
+            if (lane == 0) {   // the store that last read this space is done with it
+                if constexpr (BUFS == 2) bulk_wait_group_read1();
+                else bulk_wait_group_read0();
+            }
             __syncwarp();
+            if (staged) {
+                int8_stage_residual(ahead, stg);
+                if (i + PER < CHUNKS) int8_load_residual<T>(a, ahead, row0, nb + NC);
+                __syncwarp();
+            }
         }
+        tmem_wait_ld();
+        tmem_regs_ready(v);
+        if (i + 1 == CHUNKS) release();
+        if constexpr (EXTRA) {
+            if (a.acc && t < a.M) {
 #pragma unroll
-        for (int sub = 0; sub < SUBS; ++sub) {
-            const int c = b * NC + 32 * sub;
-            tmem_ld32(taddr + (uint32_t)c, v);
-            tmem_wait_ld();
-            tmem_regs_ready(v);
-            if (b == CW / NC - 1 && sub == SUBS - 1) release();
-            if (a.acc && t < a.M)
                 for (int j = 0; j < 32; ++j)
-                    if (n0 + c + j < a.N) {
-                        int x = 0;
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) x = i == j ? (int)v[i] : x;
-                        a.acc[(long long)t * a.ld_acc + n0 + c + j] = x;
-                    }
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {   // eight columns: 32 bytes of FP32 or 16 bytes of a shorter type
-                float f[8];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint4 al = ld_shared16(consts + (uint32_t)(c + 8 * g + 4 * h) * 4u);
-                    uint4 bi = make_uint4(0u, 0u, 0u, 0u);
-                    if (has_bias) bi = ld_shared16(consts + (uint32_t)(CW + c + 8 * g + 4 * h) * 4u);
-                    const uint32_t aw[4] = {al.x, al.y, al.z, al.w}, bw[4] = {bi.x, bi.y, bi.z, bi.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        f[4 * h + i] = int8_value<SILU>((int)v[8 * g + 4 * h + i], sq, __uint_as_float(aw[i]), has_bias,
-                                                        __uint_as_float(bw[i]));
-                }
-                constexpr int PIECES = 8 * (int)sizeof(T) / 16;   // 16-byte pieces of these eight columns
-                uint32_t at[PIECES];
-#pragma unroll
-                for (int h = 0; h < PIECES; ++h) {
-                    const int piece = (sub * 32 + 8 * g) * (int)sizeof(T) / 16 + h;
-                    at[h] = stg + (uint32_t)lane * 128u + (uint32_t)((piece ^ (lane & 7)) << 4);
-                }
-                if (a.res) {
-                    float r[8];
-                    if (p.res_vec) {
-                        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const uint4 u = ld_shared16(at[h % PIECES]);
-                                r[4 * h] = __uint_as_float(u.x);
-                                r[4 * h + 1] = __uint_as_float(u.y);
-                                r[4 * h + 2] = __uint_as_float(u.z);
-                                r[4 * h + 3] = __uint_as_float(u.w);
-                            }
-                        } else {
-                            const uint4 u = ld_shared16(at[0]);
-                            const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float2 q = unpack2<T>(uw[i]);
-                                r[2 * i] = q.x;
-                                r[2 * i + 1] = q.y;
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int n = n0 + c + 8 * g + i;
-                            r[i] = t < a.M && n < a.N ? to_float(static_cast<const T *>(a.res)[(long long)t * a.ld_res + n]) : 0.f;
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] = __fadd_rn(r[i], __fmul_rn(a.res_scale, f[i]));
-                }
-                if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        st_shared16(at[h % PIECES], __float_as_uint(f[4 * h]), __float_as_uint(f[4 * h + 1]),
-                                    __float_as_uint(f[4 * h + 2]), __float_as_uint(f[4 * h + 3]));
-                } else {
-                    st_shared16(at[0], pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
-                }
+                    if (n0 + c + j < a.N) a.acc[(long long)t * a.ld_acc + n0 + c + j] = (int)v[j];
             }
         }
-        if (p.tma_store) {
-            fence_async_shared();
-            __syncwarp();
-            if (lane == 0) {
-                if (nb < a.N && row0 < a.M) tma_store_2d(ymap, stg, nb, row0);
-                bulk_commit_group();
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+            const ulonglong2 al = ld_shared_pairs(consts + (uint32_t)(c + 4 * g) * 4u);
+            const ulonglong2 bi = ld_shared_pairs(consts + (uint32_t)(CW + c + 4 * g) * 4u);
+            float f[4];
+            unpair(int8_values<SILU>((int)v[4 * g], (int)v[4 * g + 1], sq, al.x, bi.x), f[0], f[1]);
+            unpair(int8_values<SILU>((int)v[4 * g + 2], (int)v[4 * g + 3], sq, al.y, bi.y), f[2], f[3]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * g + j] = __float_as_uint(f[j]);
+        }
+        if (has_res) {
+#pragma unroll
+            for (int h = 0; h < PIECES; ++h) {
+                float r[E];
+                if (staged) {
+                    const uint4 u = ld_shared16(rowaddr + (uint32_t)(((piece0 + h) ^ (lane & 7)) << 4));
+                    const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if constexpr (sizeof(T) == 4) {
+                            r[j] = __uint_as_float(uw[j]);
+                        } else {
+                            const float2 q = unpack2<T>(uw[j]);
+                            r[2 * j] = q.x;
+                            r[2 * j + 1] = q.y;
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < E; ++j) {
+                        const int n = n0 + c + h * E + j;
+                        r[j] = t < a.M && n < a.N ? to_float(static_cast<const T *>(a.res)[(long long)t * a.ld_res + n]) : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < E; ++j)
+                    v[h * E + j] = __float_as_uint(__fadd_rn(r[j], __fmul_rn(a.res_scale, __uint_as_float(v[h * E + j]))));
             }
-        } else {
-            __syncwarp();
-            int8_store_rows<T>(a, stg, row0, nb);
-            __syncwarp();
+        }
+#pragma unroll
+        for (int h = 0; h < PIECES; ++h) {
+            const uint32_t at = rowaddr + (uint32_t)(((piece0 + h) ^ (lane & 7)) << 4);
+            if constexpr (sizeof(T) == 4) {
+                st_shared16(at, v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+            } else {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    w[j] = pack2<T>(__uint_as_float(v[8 * h + 2 * j]), __uint_as_float(v[8 * h + 2 * j + 1]));
+                st_shared16(at, w[0], w[1], w[2], w[3]);
+            }
+        }
+        if (i % PER == PER - 1) {
+            if (p.tma_store) {
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) {
+                    if (nb < a.N && row0 < a.M) tma_store_2d(ymap, stg, nb, row0);
+                    bulk_commit_group();
+                }
+            } else {
+                __syncwarp();
+                int8_store_rows<T>(a, stg, row0, nb);
+                __syncwarp();
+            }
+            ++box;
         }
     }
 }
@@ -203,7 +207,7 @@ KEA_DEVI void int8_epilogue_tile(const Int8TileArgs &p, const CUtensorMap *ymap,
 template <> KEA_DEVI uint32_t pack2<float>(float, float) { return 0u; }
 template <> KEA_DEVI float2 unpack2<float>(uint32_t) { return make_float2(0.f, 0.f); }
 
-template <typename T, bool SILU, int CTAS, int BN>
+template <typename T, bool SILU, bool EXTRA, int CTAS, int BN>
 __global__ void __launch_bounds__(Int8Tile<CTAS, BN>::THREADS, 1)
 int8_gemm_tile_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap wmap,
                       const __grid_constant__ CUtensorMap ymap, const Int8TileArgs p) {
@@ -355,24 +359,27 @@ int8_gemm_tile_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             __syncwarp();
         }
     } else {
-        const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
+        const int ew = warp - 2, quad = warp & 3, part = ew >> 2;
         const uint32_t stg = STG0 + (uint32_t)(ew * Tile::BUFS) * kI8Box;
         const uint32_t consts = CONST0 + (uint32_t)(ew * Tile::CW) * 8u;
-        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * Tile::CW);
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(part * Tile::CW);
         int j = 0, box = 0;
         for (int tile = worker; tile < p.tiles; tile += workers, ++j) {
             const int buf = j & 1;
             const int mt = tile / p.n_tiles, nt = tile - mt * p.n_tiles;
-            const int row0 = mt * 128 * CTAS + (int)rank * 128 + quad * 32, n0 = nt * BN + half * Tile::CW;
+            const int row0 = mt * 128 * CTAS + (int)rank * 128 + quad * 32, n0 = nt * BN + part * Tile::CW;
 #pragma unroll
             for (int i = 0; i < Tile::CW; i += 32) {   // this warp's channel constants, while the accumulator fills
                 const int n = n0 + i + lane;
                 const float al = n < p.a.N ? __ldg(p.a.alpha + n) : 0.f;
-                const float bi = p.a.bias && n < p.a.N ? __ldg(p.a.bias + n) : 0.f;
+                const float bi = p.a.bias && n < p.a.N ? __ldg(p.a.bias + n) : kI8NoBias;
                 asm volatile("st.shared.f32 [%0], %1;" ::"r"(consts + (uint32_t)(i + lane) * 4u), "f"(al) : "memory");
                 asm volatile("st.shared.f32 [%0], %1;" ::"r"(consts + (uint32_t)(Tile::CW + i + lane) * 4u), "f"(bi) : "memory");
             }
-            const float sq = row0 + lane < p.a.M ? p.a.qs[row0 + lane] : 0.f;
+            const float s = row0 + lane < p.a.M ? p.a.qs[row0 + lane] : 0.f;
+            const uint64_t sq = pair_of(s, s);
+            uint4 ahead[8];
+            if (p.a.res && p.res_vec) int8_load_residual<T>(p.a, ahead, row0, n0);
             __syncwarp();
             const bool done = mbar_wait_sleep(smem_u32(&bar_acc_full[buf]), (uint32_t)((j >> 1) & 1), kOpWaitBudget, 64);
             if (!__all_sync(0xFFFFFFFFu, done)) {
@@ -381,8 +388,8 @@ int8_gemm_tile_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             }
             tc_fence_after();
             const uint32_t acc_empty = smem_u32(&bar_acc_empty[buf]);
-            int8_epilogue_tile<T, SILU, Tile::CW, Tile::BUFS>(p, &ymap, lanes + (uint32_t)(buf * BN), stg, consts, row0, n0, sq,
-                                                              box, [&] {
+            int8_epilogue_tile<T, SILU, EXTRA, Tile::CW, Tile::BUFS>(p, &ymap, lanes + (uint32_t)(buf * BN), stg, consts, row0, n0, sq,
+                                                              box, ahead, [&] {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
