@@ -7,7 +7,10 @@
 //
 // `tpr` threads (32 .. 512) hold one row in registers, VPT values each, so every input is read and every output written
 // once; a LayerNorm takes two group sums (mean, then centred squares), a root-mean-square norm one, the codes one maximum.
-// VEC: eight consecutive values per chunk (32-byte FP32 or 16-byte loads); otherwise thread i holds values i, i + tpr, ...
+// VEC: whole vectors per chunk; otherwise thread i holds values i, i + tpr, ...
+//
+// Two kernels: residual_norm_kernel for rows at any stride, a group of threads to a row; residual_norm_flat_kernel (below) for
+// many contiguous rows whose width no vector fits.
 #pragma once
 
 #include "operator_common.cuh"
@@ -36,33 +39,54 @@ constexpr int kRnThreads = 256;
 constexpr int kRnMaxThreads = 512;
 constexpr int kRnSlots = 5;   // group reductions of one launch
 
-KEA_DEVI void load8(const float *p, float *v) {
-    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
-                 : "l"(p)
-                 : "memory");
-}
-template <typename T>
-KEA_DEVI void load8(const T *p, float *v) {
-    const uint4 w = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+// W consecutive values (1, or whole vectors of 4 or 8) to and from FP32 registers.
+template <int W, typename T>
+KEA_DEVI void get(const T *p, float *v) {
+    if constexpr (W == 1) {
+        v[0] = to_float(*p);
+    } else if constexpr (sizeof(T) == 4 && W == 8) {   // a 32-byte load; ordered after griddepcontrol.wait (volatile)
+        asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                     : "l"(p));
+    } else if constexpr (sizeof(T) == 4) {
+        const float4 f = *reinterpret_cast<const float4 *>(p);
+        v[0] = f.x;
+        v[1] = f.y;
+        v[2] = f.z;
+        v[3] = f.w;
+    } else {
+        uint32_t u[W / 2];
+        if constexpr (W == 8) *reinterpret_cast<uint4 *>(u) = *reinterpret_cast<const uint4 *>(p);
+        else *reinterpret_cast<uint2 *>(u) = *reinterpret_cast<const uint2 *>(p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack2<T>(u[i]);
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+        for (int i = 0; i < W / 2; ++i) {
+            const float2 f = unpack2<T>(u[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
     }
 }
-KEA_DEVI void store8(float *p, const float *v) {
-    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]),
-                 "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
-                 : "memory");
+template <int W, typename T>
+KEA_DEVI void put(T *p, const float *v) {
+    if constexpr (W == 1) {
+        *p = from_float<T>(v[0]);
+    } else if constexpr (sizeof(T) == 4 && W == 8) {
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+                     "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                     : "memory");
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+        uint32_t u[W / 2];
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) u[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+        if constexpr (W == 8) *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(u);
+        else *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(u);
+    }
 }
-template <typename T>
-KEA_DEVI void store8(T *p, const float *v) {
-    *reinterpret_cast<uint4 *>(p) =
-        make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
-}
+// float has no 16-bit packing; never called
+template <> KEA_DEVI uint32_t pack2<float>(float, float) { return 0u; }
+template <> KEA_DEVI float2 unpack2<float>(uint32_t) { return make_float2(0.f, 0.f); }
 
 // Sum or maximum over a row group's threads in a fixed order; `slot`: kRnMaxThreads / 32 floats used by this reduction
 // alone. Every thread of the CTA calls it.
@@ -83,145 +107,343 @@ KEA_DEVI float row_reduce(float v, int tpr, float *slot) {
     return r;
 }
 
-template <typename TX, typename TY, int VPT, bool VEC>
-struct RowStep {
-    static constexpr int C = VEC ? VPT / 8 : VPT, W = VEC ? 8 : 1;
+// One thread's share of a row: VPT values in chunks of W, chunk c at (c * tpr + gt) * W. Nothing here branches on a chunk
+// being inside the row: chunks past its end read the last one and count as zeros (a branch per chunk would make every
+// chunk wait for its own loads: rows of 1001 values took six times as long).
+template <int VPT, int W>
+struct RowPart {
+    static constexpr int C = VPT / W;
     int gt, tpr, D;
-    KEA_DEVI int at(int c) const { return (c * tpr + gt) * W; }   // first value of chunk c
+    KEA_DEVI int at(int c) const { return (c * tpr + gt) * W; }
     KEA_DEVI bool in(int c) const { return at(c) < D; }
+    KEA_DEVI int safe(int c) const { return min(at(c), D - W); }
 
     template <typename T>
     KEA_DEVI void load(const T *row, float (&v)[VPT]) const {
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            if (in(c)) {
-                if constexpr (VEC) load8(row + at(c), v + 8 * c);
-                else v[c] = to_float(row[at(c)]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < W; ++i) v[W * c + i] = 0.f;
-            }
-        }
-    }
-    template <typename T>
-    KEA_DEVI void store(T *row, const float (&v)[VPT]) const {
+        for (int c = 0; c < C; ++c) get<W>(row + safe(c), v + W * c);
 #pragma unroll
         for (int c = 0; c < C; ++c)
-            if (in(c)) {
-                if constexpr (VEC) store8(row + at(c), v + 8 * c);
-                else row[at(c)] = from_float<T>(v[c]);
-            }
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[W * c + i] = in(c) ? v[W * c + i] : 0.f;
+    }
+    template <typename T>
+    KEA_DEVI void store(T *row, const float (&v)[VPT], bool live) const {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            if (live && in(c)) put<W>(row + at(c), v + W * c);
     }
     KEA_DEVI void norm(float (&v)[VPT], int kind, const float *w, const float *b, float eps, float *slots) const {
-        float mean = 0.f;
         if (kind == KEA_NORM_LAYER) {
             float s = 0.f;
 #pragma unroll
             for (int i = 0; i < VPT; ++i) s += v[i];
-            mean = __fdiv_rn(row_reduce<false>(s, tpr, slots), (float)D);
+            const float mean = __fdiv_rn(row_reduce<false>(s, tpr, slots), (float)D);
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[W * c + i] = in(c) ? v[W * c + i] - mean : 0.f;
         }
         float ss = 0.f;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-            if (in(c)) {
-#pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    v[W * c + i] -= mean;
-                    ss = fmaf(v[W * c + i], v[W * c + i], ss);
-                }
-            }
+        for (int i = 0; i < VPT; ++i) ss = fmaf(v[i], v[i], ss);
         const float inv = rsqrtf(__fdiv_rn(row_reduce<false>(ss, tpr, slots + kRnMaxThreads / 32), (float)D) + eps);
+        if (b) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float wv[W], bv[W];
+                get<W>(w + safe(c), wv);
+                get<W>(b + safe(c), bv);
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[W * c + i] = fmaf(v[W * c + i] * inv, wv[i], bv[i]);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float wv[W];
+                get<W>(w + safe(c), wv);
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[W * c + i] = v[W * c + i] * inv * wv[i];
+            }
+        }
+    }
+    template <typename T>
+    KEA_DEVI void gate(float (&v)[VPT], const T *g, int act) const {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float gv[W];
+            get<W>(g + safe(c), gv);
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                if (act == KEA_GATE_SIGMOID) gv[i] = __fdividef(1.0f, 1.0f + __expf(-gv[i]));
+                v[W * c + i] *= gv[i];
+            }
+        }
+    }
+    // h as INT8 codes with one scale, as the quantizer's single part
+    KEA_DEVI void codes(const float (&v)[VPT], int8_t *q, int ldq, float *qs, bool live, float *slot) const {
+        float amax = 0.f;
 #pragma unroll
         for (int c = 0; c < C; ++c)
-            if (in(c)) {
-                float wv[W], bv[W];
-                if constexpr (VEC) {
-                    load8(w + at(c), wv);
-                    if (b) load8(b + at(c), bv);
-                } else {
-                    wv[0] = w[at(c)];
-                    if (b) bv[0] = b[at(c)];
-                }
 #pragma unroll
-                for (int i = 0; i < W; ++i) v[W * c + i] = fmaf(v[W * c + i] * inv, wv[i], b ? bv[i] : 0.f);
+            for (int i = 0; i < W; ++i) amax = fmaxf(amax, in(c) ? fabsf(v[W * c + i]) : 0.f);
+        amax = row_reduce<true>(amax, tpr, slot);
+        const float s = fmaxf(__fdiv_rn(amax, 127.0f), 1.0e-30f), inv = __frcp_rn(s);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if constexpr (W == 1) {
+                if (live && in(c)) q[at(c)] = (int8_t)(int)round_quotient(v[c], s, inv);
+            } else {
+                float t[4];
+                uint32_t word[W / 4];
+#pragma unroll
+                for (int h = 0; h < W / 4; ++h) word[h] = quantize4(v + W * c + 4 * h, s, inv, t);
+                if (live && in(c)) {
+                    if constexpr (W == 8) *reinterpret_cast<uint2 *>(q + at(c)) = make_uint2(word[0], word[1]);
+                    else *reinterpret_cast<uint32_t *>(q + at(c)) = word[0];
+                }
             }
+        }
+        if (live) {
+            for (int e = D + gt; e < ldq; e += tpr) q[e] = 0;   // padding columns
+            if (gt == 0) *qs = s;
+        }
     }
 };
 
 template <typename TX, typename TY, int VPT, bool VEC>
 __global__ void __launch_bounds__(kRnMaxThreads) residual_norm_kernel(const ResidualNormArgs a, int tpr) {
     __shared__ float slots[kRnSlots * (kRnMaxThreads / 32)];
+    constexpr int S = kRnMaxThreads / 32, W = VEC ? 8 : 1;
     const int rows = blockDim.x / tpr;
-    const int m = blockIdx.x * rows + threadIdx.x / tpr;
-    const bool live = m < a.M;
-    const RowStep<TX, TY, VPT, VEC> row{(int)(threadIdx.x % tpr), tpr, live ? a.D : 0};
-    using Row = RowStep<TX, TY, VPT, VEC>;
-    const long long mr = live ? m : 0;
+    const int row = blockIdx.x * rows + threadIdx.x / tpr;
+    const bool live = row < a.M;
+    const long long m = live ? row : a.M - 1;   // a group past the last row does that one again and stores nothing
+    const RowPart<VPT, W> part{(int)(threadIdx.x % tpr), tpr, a.D};
     grid_dependency_wait();
     grid_launch_dependents();
     float u[VPT], x[VPT];
-    row.load(static_cast<const TY *>(a.y) + mr * a.ldy, u);
-    row.load(static_cast<const TX *>(a.x) + mr * a.ldx, x);
-    constexpr int S = kRnMaxThreads / 32;
-    RowStep<TX, TY, VPT, VEC> full = row;
-    full.D = a.D;   // statistics divide by the row's width; a dead group's values are zeros
-    if (a.post) full.norm(u, a.post, a.post_w, a.post_b, a.post_eps, slots);
-    if (a.gate) {
-        const TY *gate = static_cast<const TY *>(a.gate) + (mr / a.frames) * a.gate_clip + (mr % a.frames) * a.gate_row;
+    part.load(static_cast<const TY *>(a.y) + m * a.ldy, u);
+    part.load(static_cast<const TX *>(a.x) + m * a.ldx, x);
+    if (a.post) part.norm(u, a.post, a.post_w, a.post_b, a.post_eps, slots);
+    if (a.gate)
+        part.gate(u, static_cast<const TY *>(a.gate) + m / a.frames * a.gate_clip + m % a.frames * a.gate_row, a.gate_act);
+    // in place, the last row is still to be read by the groups that do it again
+    if (a.r == a.x && (blockIdx.x + 1) * rows > a.M) __syncthreads();
 #pragma unroll
-        for (int c = 0; c < Row::C; ++c)
-            if (row.in(c)) {
-                float g[Row::W];
-                if constexpr (VEC) load8(gate + row.at(c), g);
-                else g[0] = to_float(gate[row.at(c)]);
+    for (int c = 0; c < VPT / W; ++c)
 #pragma unroll
-                for (int i = 0; i < Row::W; ++i) {
-                    if (a.gate_act == KEA_GATE_SIGMOID) g[i] = __fdividef(1.0f, 1.0f + __expf(-g[i]));
-                    u[Row::W * c + i] *= g[i];
-                }
-            }
-    }
-#pragma unroll
-    for (int c = 0; c < Row::C; ++c)
-        if (row.in(c)) {
-#pragma unroll
-            for (int i = 0; i < Row::W; ++i) x[Row::W * c + i] = fmaf(a.scale, u[Row::W * c + i], x[Row::W * c + i]);
-        }
-    row.store(static_cast<TX *>(a.r) + mr * a.ldr, x);
-    if (a.pre) full.norm(x, a.pre, a.pre_w, a.pre_b, a.pre_eps, slots + 2 * S);
+        for (int i = 0; i < W; ++i) x[W * c + i] = part.in(c) ? fmaf(a.scale, u[W * c + i], x[W * c + i]) : 0.f;
+    part.store(static_cast<TX *>(a.r) + m * a.ldr, x, live);
+    if (a.pre) part.norm(x, a.pre, a.pre_w, a.pre_b, a.pre_eps, slots + 2 * S);
     if (a.h) {
-        if (a.h_type == KEA_TYPE_F32) row.store(static_cast<float *>(a.h) + mr * a.ldh, x);
-        else if (a.h_type == KEA_TYPE_F16) row.store(static_cast<__half *>(a.h) + mr * a.ldh, x);
-        else row.store(static_cast<__nv_bfloat16 *>(a.h) + mr * a.ldh, x);
+        if (a.h_type == KEA_TYPE_F32) part.store(static_cast<float *>(a.h) + m * a.ldh, x, live);
+        else if (a.h_type == KEA_TYPE_F16) part.store(static_cast<__half *>(a.h) + m * a.ldh, x, live);
+        else part.store(static_cast<__nv_bfloat16 *>(a.h) + m * a.ldh, x, live);
     }
-    if (a.q) {
-        float amax = 0.f;
+    if (a.q) part.codes(x, a.q + m * a.ldq, a.ldq, a.qs + m, live, slots + 4 * S);
+}
+
+// ---- many contiguous rows of any width -----------------------------------------------------------------------------------
+// Rows whose width is no multiple of eight start at any address. Read value by value they cost a memory instruction per 32
+// values (12024 rows of 1001 values, FP32 stream and BF16 block: 66 us in registers, 79 and 136 us through shared memory,
+// against 22 us of traffic; 3000 instructions a row bound it). But in one contiguous buffer the groups of eight values
+// that start at a multiple of eight are aligned in x, y, r, h and a gate of x's shape alike, wherever the rows begin: a
+// thread takes such groups, the two at a row's ends in part. What does not line up is the parameters: value i of a row
+// sits in its group at (i + o) % 8 with the row's own o. They are held in shared memory four times, shifted by 0 .. 3
+// values, so that every group finds its parameters in two aligned vectors of one of the copies. One CTA of 16 warps per
+// SM shares the copies and takes rows in turn.
+constexpr int kFlatThreads = 512, kFlatVpt = 32, kFlatGroups = kFlatVpt / 8;
+
+struct FlatArgs {
+    ResidualNormArgs a;
+    int padded;               // floats of one shifted copy: whole rows of groups and eight more
+    int params;               // bit k: parameter k (post weight, post bias, pre weight, pre bias, shared gate) is held
+};
+
+// Eight values of a row: groups of the flat buffer, `lo` .. `hi` of each inside the row.
+template <int TPR>
+struct FlatRow {
+    long long first;          // flat index of this thread's first group
+    long long total;
+    int i0, D;                // index in the row of that group's first value (negative before the row)
+    KEA_DEVI int index(int c) const { return i0 + 8 * TPR * c; }
+    KEA_DEVI bool whole(int c) const { return index(c) >= 0 && index(c) + 8 <= D; }
+    KEA_DEVI bool some(int c) const { return index(c) + 8 > 0 && index(c) < D; }
+    KEA_DEVI bool has(int c, int e) const { return (unsigned)(index(c) + e) < (unsigned)D; }
+
+    template <typename T>
+    KEA_DEVI void load(const T *p, float (&v)[kFlatVpt]) const {
 #pragma unroll
-        for (int c = 0; c < Row::C; ++c)
-            if (row.in(c)) {
+        for (int c = 0; c < kFlatGroups; ++c) {
+            const long long f = first + 8LL * TPR * c;
+            if (f + 8 <= total) {
+                get<8>(p + f, v + 8 * c);
+            } else {   // the buffer's end
 #pragma unroll
-                for (int i = 0; i < Row::W; ++i) amax = fmaxf(amax, fabsf(x[Row::W * c + i]));
+                for (int e = 0; e < 8; ++e) v[8 * c + e] = f + e < total ? to_float(p[f + e]) : 0.f;
             }
-        amax = row_reduce<true>(amax, tpr, slots + 4 * S);
-        const float s = fmaxf(__fdiv_rn(amax, 127.0f), 1.0e-30f), inv = __frcp_rn(s);
-        int8_t *q = a.q + mr * a.ldq;
+        }
+    }
+    KEA_DEVI void clear(float (&v)[kFlatVpt]) const {   // zeros where a group reaches out of the row
 #pragma unroll
-        for (int c = 0; c < Row::C; ++c)
-            if (row.in(c)) {
-                if constexpr (VEC) {
-                    float t[4];
-                    uint2 w;
-                    w.x = quantize4(x + 8 * c, s, inv, t);
-                    w.y = quantize4(x + 8 * c + 4, s, inv, t);
-                    *reinterpret_cast<uint2 *>(q + row.at(c)) = w;
-                } else {
-                    q[row.at(c)] = (int8_t)(int)round_quotient(x[c], s, inv);
+        for (int c = 0; c < kFlatGroups; ++c)
+            if (!whole(c)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[8 * c + e] = has(c, e) ? v[8 * c + e] : 0.f;
+            }
+    }
+    template <typename T>
+    KEA_DEVI void store(T *p, const float (&v)[kFlatVpt]) const {
+#pragma unroll
+        for (int c = 0; c < kFlatGroups; ++c) {
+            T *const at = p + first + 8LL * TPR * c;
+            if (whole(c)) {
+                put<8>(at, v + 8 * c);
+            } else if (some(c)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (has(c, e)) at[e] = from_float<T>(v[8 * c + e]);
+            }
+        }
+    }
+    // `w`: this row's shifted copy at this thread's first group
+    KEA_DEVI static void scaled(float (&v)[kFlatVpt], float by, const float *w, const float *b) {
+#pragma unroll
+        for (int c = 0; c < kFlatGroups; ++c) {
+            float wv[8], bv[8];
+            get<4>(w + 8 * TPR * c, wv);
+            get<4>(w + 8 * TPR * c + 4, wv + 4);
+            if (b) {
+                get<4>(b + 8 * TPR * c, bv);
+                get<4>(b + 8 * TPR * c + 4, bv + 4);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float t = v[8 * c + e] * by;
+                v[8 * c + e] = b ? fmaf(t, wv[e], bv[e]) : t * wv[e];
+            }
+        }
+    }
+    KEA_DEVI void norm(float (&v)[kFlatVpt], int kind, float eps, const float *w, const float *b, float *slots) const {
+        if (kind == KEA_NORM_LAYER) {
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < kFlatVpt; ++i) s += v[i];
+            const float mean = __fdiv_rn(row_reduce<false>(s, TPR, slots), (float)D);
+#pragma unroll
+            for (int i = 0; i < kFlatVpt; ++i) v[i] -= mean;
+            clear(v);
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < kFlatVpt; ++i) ss = fmaf(v[i], v[i], ss);
+        const float inv = rsqrtf(__fdiv_rn(row_reduce<false>(ss, TPR, slots + kRnMaxThreads / 32), (float)D) + eps);
+        scaled(v, inv, w, b);
+    }
+};
+
+template <typename TX, typename TY, int TPR>
+__global__ void __launch_bounds__(kFlatThreads, 1) residual_norm_flat_kernel(const __grid_constant__ FlatArgs p) {
+    extern __shared__ __align__(16) float copies[];   // [held parameters][4 shifts][padded]
+    __shared__ float slots[kRnSlots * (kRnMaxThreads / 32)];
+    constexpr int SL = kRnMaxThreads / 32, GROUPS = kFlatThreads / TPR;
+    const ResidualNormArgs &a = p.a;
+    const int D = a.D, group = (int)threadIdx.x / TPR, gt = (int)threadIdx.x % TPR;
+    const long long total = (long long)a.M * D;
+    const float *const source[4] = {a.post_w, a.post_b, a.pre_w, a.pre_b};
+    const float *held[5];
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < 5; ++k) {
+        held[k] = nullptr;
+        if (p.params >> k & 1) held[k] = copies + (size_t)4 * p.padded * n++;
+    }
+    // copy s holds value i at i + 8 + s: the group with row index i0 = 8 t - o finds its values at i0 + 8 + (o % 4)
+    const auto fill = [&](float *to, auto value) {
+        for (int i = threadIdx.x; i < 4 * p.padded; i += kFlatThreads) {
+            const int s = i / p.padded, at = i - s * p.padded - 8 - s;
+            to[i] = at >= 0 && at < D ? value(at) : 0.f;
+        }
+    };
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (held[k]) fill(const_cast<float *>(held[k]), [&](int i) { return __ldg(source[k] + i); });
+    grid_dependency_wait();
+    grid_launch_dependents();
+    if (held[4])
+        fill(const_cast<float *>(held[4]), [&](int i) {
+            const float g = to_float(static_cast<const TY *>(a.gate)[i]);
+            return a.gate_act == KEA_GATE_SIGMOID ? __fdividef(1.0f, 1.0f + __expf(-g)) : g;
+        });
+    __syncthreads();
+
+    const int turns = (a.M + (int)gridDim.x * GROUPS - 1) / ((int)gridDim.x * GROUPS);
+    for (int turn = 0; turn < turns; ++turn) {   // every thread takes every turn (row_reduce has barriers)
+        const long long wanted = ((long long)turn * gridDim.x + blockIdx.x) * GROUPS + group;
+        const bool live = wanted < a.M;
+        if (TPR == 32 && !live) break;
+        const int m = live ? (int)wanted : 0;
+        const long long start = (long long)m * D;
+        const int o = (int)(start & 7);
+        const FlatRow<TPR> row{start - o + 8LL * gt, total, 8 * gt - o, D};
+        const int at = row.i0 + 8 + (o & 3);   // of this thread's first group in the row's copy, a multiple of four
+        const auto mine = [&](int k) { return held[k] ? held[k] + (o & 3) * p.padded + at : nullptr; };
+        float u[kFlatVpt], x[kFlatVpt];
+        row.load(static_cast<const TY *>(a.y), u);
+        row.load(static_cast<const TX *>(a.x), x);
+        row.clear(u);
+        if (a.post) row.norm(u, a.post, a.post_eps, mine(0), mine(1), slots);
+        if (held[4]) {
+            row.scaled(u, 1.0f, mine(4), nullptr);
+        } else if (a.gate) {
+            float g[kFlatVpt];
+            if (a.gate_row == D && a.gate_clip == (long long)a.frames * D) {
+                row.load(static_cast<const TY *>(a.gate), g);
+            } else {   // one row per clip: value by value
+                const TY *const gr = static_cast<const TY *>(a.gate) + (long long)(m / a.frames) * a.gate_clip + (long long)(m % a.frames) * a.gate_row;
+#pragma unroll
+                for (int c = 0; c < kFlatGroups; ++c)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) g[8 * c + e] = row.has(c, e) ? to_float(gr[row.index(c) + e]) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < kFlatVpt; ++i) u[i] *= a.gate_act == KEA_GATE_SIGMOID ? __fdividef(1.0f, 1.0f + __expf(-g[i])) : g[i];
+        }
+#pragma unroll
+        for (int i = 0; i < kFlatVpt; ++i) x[i] = fmaf(a.scale, u[i], x[i]);
+        row.clear(x);
+        if (live) row.store(static_cast<TX *>(a.r), x);
+        if (a.pre) row.norm(x, a.pre, a.pre_eps, mine(2), mine(3), slots + 2 * SL);
+        if (a.h && live) {
+            if (a.h_type == KEA_TYPE_F32) row.store(static_cast<float *>(a.h), x);
+            else if (a.h_type == KEA_TYPE_F16) row.store(static_cast<__half *>(a.h), x);
+            else row.store(static_cast<__nv_bfloat16 *>(a.h), x);
+        }
+        if (a.q) {   // codes with one scale, as the quantizer's single part
+            row.clear(x);
+            float amax = 0.f;
+#pragma unroll
+            for (int i = 0; i < kFlatVpt; ++i) amax = fmaxf(amax, fabsf(x[i]));
+            amax = row_reduce<true>(amax, TPR, slots + 4 * SL);
+            const float s = fmaxf(__fdiv_rn(amax, 127.0f), 1.0e-30f), inv = __frcp_rn(s);
+            int8_t *const q = a.q + (long long)m * a.ldq;
+#pragma unroll
+            for (int c = 0; c < kFlatGroups; ++c) {
+                float t[4];
+                const uint32_t word[2] = {quantize4(x + 8 * c, s, inv, t), quantize4(x + 8 * c + 4, s, inv, t)};
+                if (live && row.some(c)) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (row.has(c, e)) q[row.index(c) + e] = (int8_t)(word[e / 4] >> (8 * (e % 4)));
                 }
             }
-        if (live) {
-            for (int i = a.D + row.gt; i < a.ldq; i += tpr) q[i] = 0;   // padding columns
-            if (row.gt == 0) a.qs[m] = s;
+            if (live) {
+                for (int e = D + gt; e < a.ldq; e += TPR) q[e] = 0;   // padding columns
+                if (gt == 0) a.qs[m] = s;
+            }
         }
+        if (TPR > 32) __syncthreads();   // the reductions' slots serve the next rows
     }
 }
 

@@ -2,7 +2,9 @@
 
 Tolerances. A row's sums run over at most 32 values per thread and 14 levels of adding up, so a mean, a mean square or the
 value normed with it is off by at most about 50 * 2^-24 = 3e-6 of the row's largest value; two norms and the step between
-make that 1e-5 (the rows' spread is at least 0.3, so a norm does not enlarge it by more than 4). A shorter type adds half
+make that 1e-5 where the second norm does not enlarge what reaches it by more than 4: it divides by the row's spread, so
+where the terms of r are more than 4 times that (rows of one value, near zero by cancellation) the bound on h grows with
+them (`_enlarged`). A shorter type adds half
 a unit in its last place. INT8 codes may differ by one where the value lies within that of the middle between two."""
 from __future__ import annotations
 
@@ -47,8 +49,16 @@ def _exact(x, y, post, gate, act, scale, pre):
     return r, _exact_norm(r, pre)
 
 
-def _near(got, want):
-    tol = 1e-5 * want.abs().amax(-1, keepdim=True).clamp_min(1.0)
+def _enlarged(x, r, pre):
+    """How much more than 4 times pre enlarges an error of r's terms, per row."""
+    x = x.cpu().double()
+    size = (x.abs() + (r - x).abs()).amax(-1, keepdim=True)
+    v = r - r.mean(-1, keepdim=True) if isinstance(pre, nn.LayerNorm) else r
+    return (size / ((v * v).mean(-1, keepdim=True) + pre.eps).sqrt() / 4.0).clamp_min(1.0)
+
+
+def _near(got, want, enlarged=1.0):
+    tol = 1e-5 * want.abs().amax(-1, keepdim=True).clamp_min(1.0) * enlarged
     if got.dtype != F32:
         tol = tol + 2.0 ** (-11 if got.dtype == F16 else -8) * (want.abs() + tol) + (2.0 ** -25 if got.dtype == F16 else 0.0)
     off = (got.cpu().double() - want).abs()
@@ -87,6 +97,27 @@ def test_widths_and_row_counts(rows, d):
     want_r, want_h = _exact(x, y, post, gt, "none", 1.0, pre)
     _near(r, want_r)
     _near(h, want_h)
+
+
+@pytest.mark.parametrize("tx,ty,th", [(F32, F32, F32), (F32, BF16, BF16), (BF16, F16, BF16), (F16, F32, F16)])
+@pytest.mark.parametrize("shape,gate", [((1, 9001, 1), "row"), ((3, 1667, 7), "channel"), ((2, 2501, 33), "clip"), ((1, 4999, 100), "row"),
+                                        ((5, 600, 257), "row"), ((1, 2999, 513), "channel"), ((3, 1001, 1001), "clip"),
+                                        ((1, 2400, 1023), "row"), ((1, 1501, 2047), None), ((7, 101, 4095), "clip"), ((1, 9001, 1024), "row")])
+def test_many_rows(shape, gate, tx, ty, th):
+    """Rows enough for every SM, of widths that no vector fits, the last group of rows short; in place and not."""
+    d = shape[-1]
+    x, y, gt, g = _inputs(shape, tx, ty, seed=d, gate=gate)
+    post, pre = _norm("rms", d, g), _norm("layer" if d > 8 else "rms", d, g)
+    want_r, want_h = _exact(x, y, post, gt, "sigmoid", 0.5, pre)
+    r, h = lowbit.residual_norm(x, y, post_norm=post, gate=gt, gate_act="sigmoid", scale=0.5, pre_norm=pre, dtype=th)
+    _near(r, want_r)
+    more = _enlarged(x, want_r, pre)
+    _near(h, want_h, more)
+    q, qs = lowbit.residual_norm_quantized(x, y, post_norm=post, gate=gt, gate_act="sigmoid", scale=0.5, pre_norm=pre, out=x)[1:]
+    assert torch.equal(x, r)
+    steps = want_h.reshape(-1, d) / qs.cpu().double()[:, None]
+    assert bool(((q.cpu().double() - steps).abs() <= 0.5 + 127 * 2e-5 * 4 * more.reshape(-1, 1)).all())
+    assert _lib.read_device_error() == 0
 
 
 @pytest.mark.parametrize("d", [96, 100, 1001])
