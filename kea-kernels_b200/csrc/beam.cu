@@ -1,5 +1,6 @@
 // beam.cu - host side of the beam-search step: kea_lowbit_beam_select and kea_lowbit_beam_reorder.
 #include <algorithm>
+#include <atomic>
 
 #include "beam_kernels.cuh"
 #include "host.h"
@@ -28,12 +29,19 @@ int validate(const KeaBeamDesc *d) {
     return KEA_OK;
 }
 
-template <typename T>
-cudaError_t launch_select(const kea::BeamArgs &a, int clips, bool pdl, void *stream) {
+template <typename T, int WARPS>
+cudaError_t launch_select_as(const kea::BeamArgs &a, int clips, int device, bool pdl, void *stream) {
+    const auto kernel = kea::beam_select_kernel<T, WARPS>;
+    static std::atomic<uint64_t> ready{0};   // devices on which clusters of 16 are allowed
+    if (a.ctas > 8 && !(ready.load(std::memory_order_acquire) >> device & 1)) {
+        const cudaError_t e = cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+        ready.fetch_or(1ULL << device, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attrs[2];
     cfg.gridDim = dim3((unsigned)(a.ctas * clips), 1, 1);
-    cfg.blockDim = dim3(kea::kBeamThreads, 1, 1);
+    cfg.blockDim = dim3(32 * WARPS, 1, 1);
     cfg.stream = (cudaStream_t)stream;
     cfg.attrs = attrs;
     if (a.ctas > 1) {
@@ -48,7 +56,12 @@ cudaError_t launch_select(const kea::BeamArgs &a, int clips, bool pdl, void *str
         attrs[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
         ++cfg.numAttrs;
     }
-    return cudaLaunchKernelEx(&cfg, kea::beam_select_kernel<T>, a);
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+template <typename T>
+cudaError_t launch_select(const kea::BeamArgs &a, int clips, int warps, int device, bool pdl, void *stream) {
+    return warps == 8 ? launch_select_as<T, 8>(a, clips, device, pdl, stream) : launch_select_as<T, 32>(a, clips, device, pdl, stream);
 }
 
 }  // namespace
@@ -73,20 +86,20 @@ extern "C" int kea_lowbit_beam_select(const KeaBeamDesc *d, void *stream) {
     a.vocab = d->vocab;
     a.width = d->width;
     a.end = d->end;
-    // CTAs per clip: until every SM has two of them, as long as each warp keeps a few hundred logits
-    int ctas = 1;
-    while (ctas < kea::kBeamCluster && (long long)ctas * d->clips < 2LL * dev.sms &&
-           (long long)d->beams * d->vocab >= 2LL * ctas * kea::kBeamWarps * 512)
-        ctas *= 2;
-    a.ctas = ctas;
-    const int warps = ctas * kea::kBeamWarps;
-    a.segs = std::max(1, warps / d->beams);
+    // Warps per clip: as many as the SMs hold at once (32 each), as long as each keeps some 512 logits; in CTAs of 8,
+    // or of 32 where a cluster of 16 of those is not enough.
+    const long long wanted = std::min((long long)d->beams * d->vocab / 512, 32LL * dev.sms / d->clips);
+    const int warps = wanted <= 8 * kea::kBeamCluster ? 8 : 32;
+    a.ctas = 1;
+    while (a.ctas < kea::kBeamCluster && 2LL * a.ctas * warps <= wanted) a.ctas *= 2;
+    const int all = a.ctas * warps;
+    a.segs = std::max(1, all / d->beams);
     a.units = a.segs * d->beams;
-    a.rounds = ceil_div(a.units, warps);
+    a.rounds = ceil_div(a.units, all);
     const bool pdl = (d->flags & KEA_BEAM_PDL) != 0;
-    const cudaError_t e = d->logits_type == KEA_TYPE_F32   ? launch_select<float>(a, d->clips, pdl, stream)
-                          : d->logits_type == KEA_TYPE_F16 ? launch_select<__half>(a, d->clips, pdl, stream)
-                                                           : launch_select<__nv_bfloat16>(a, d->clips, pdl, stream);
+    const cudaError_t e = d->logits_type == KEA_TYPE_F32   ? launch_select<float>(a, d->clips, warps, dev.index, pdl, stream)
+                          : d->logits_type == KEA_TYPE_F16 ? launch_select<__half>(a, d->clips, warps, dev.index, pdl, stream)
+                                                           : launch_select<__nv_bfloat16>(a, d->clips, warps, dev.index, pdl, stream);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return KEA_ERR_CUDA;

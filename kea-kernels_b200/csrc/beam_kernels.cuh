@@ -2,17 +2,20 @@
 // reordering of the hypotheses' states.
 //
 // Selection. c[k, v] = score_k + (x[k, v] - lse_k), lse_k = log sum_v exp x[k, v]. Within a hypothesis c falls with x, so
-// its `width` largest logits are all it can contribute, and they can be found in the same pass that sums the
-// exponentials, before lse_k is known: the logits are read once. One thread-block cluster serves a clip; each of its
-// warps takes a unit (a hypothesis, or a segment of one) and keeps, while it streams the logits,
+// its `width` largest logits are all it can contribute, and they can be found while the exponentials are summed, before
+// lse_k is known. One thread-block cluster serves a clip; each of its warps takes a unit (a hypothesis, or a segment of
+// one) and streams its logits once, a tile ahead, keeping
 //   * per lane a running maximum m and the sum of 2^(x log2 e - off), off = m log2 e rounded, in FP32; the log-sum is
 //     (off + log2 of the sum) / log2 e, so the rounding of off cancels. Where that is not finite - a logit that is not a
 //     number, or one so large that off overflows - the unit is summed again with its maximum known, masking what is not
 //     a number;
-//   * across its lanes the unit's best logits, lane i the i-th best with its index. A logit enters only if it is above
-//     the last of them, which after the first few hundred values is rare, so the common path is one maximum per value and
-//     one vote per tile. Where many lanes of a tile pass, the width-th largest of the lane maxima is a bound below which
-//     no value of the tile can enter.
+//   * the maximum of every tile.
+// The width-th largest of the lane maxima of all the CTA's warps at a hypothesis bounds its best logits from below: only
+// the few tiles whose maximum reaches it are read again (from the caches), and what reaches it in them, a little more
+// than `width` values in all, enters the warp's list. (Keeping the lists up to date while streaming made every warp pay
+// for its own `width` best: 3300 instructions for 2048 logits, 4096 x 8 x 131072 FP32 logits 43 us.) Candidates are
+// gathered in shared memory and enter 32 at a time: every lane counts how many candidates and list entries are ahead of
+// its own, independent comparisons.
 // The units' sums and lists meet in the first CTA of the cluster (distributed shared memory), which forms every lse_k and
 // merges the lists by (c, flat index). No scratch memory, one launch.
 #pragma once
@@ -21,11 +24,9 @@
 
 namespace kea {
 
-constexpr int kBeamThreads = 256, kBeamWarps = 8;
 constexpr int kBeamMax = 32;          // hypotheses and width
-constexpr int kBeamCluster = 8;       // CTAs per clip at most
-constexpr int kBeamRounds = 4;        // units per warp at most: kBeamMax hypotheses / 8 warps
-constexpr int kBeamNone = 0x7FFFFFFF; // index of an empty place
+constexpr int kBeamCluster = 16;      // CTAs per clip at most
+constexpr int kBeamSlots = 32;        // units per CTA at most: 32 hypotheses, or 32 warps with one each
 
 struct BeamArgs {
     const void *logits;
@@ -40,47 +41,72 @@ struct BeamArgs {
     int segs, units, rounds;          // segments per hypothesis, beams * segs, units per warp
 };
 
-// Order of the list: larger values first, equal ones by index.
-KEA_DEVI bool beam_before(float av, int ai, float bv, int bi) { return av > bv || (av == bv && ai < bi); }
-
-// Enters (v, i) (the same in every lane) into the warp's sorted list, lane j holding the j-th.
-KEA_DEVI void beam_insert(float v, int i, int lane, float &lv, int &li) {
-    const uint32_t ahead = __ballot_sync(0xFFFFFFFFu, beam_before(lv, li, v, i));
-    const int pos = __popc(ahead);
-    const float uv = __shfl_up_sync(0xFFFFFFFFu, lv, 1);
-    const int ui = __shfl_up_sync(0xFFFFFFFFu, li, 1);
-    if (lane > pos) {
-        lv = uv;
-        li = ui;
-    } else if (lane == pos) {
-        lv = v;
-        li = i;
-    }
-}
-
-// An unsigned key in the order of the floats (no NaN).
+// An unsigned key in the order of the floats (no NaN; -0 as 0).
 KEA_DEVI uint32_t float_key(float v) {
-    const uint32_t u = __float_as_uint(v);
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    const uint32_t u = __float_as_uint(v + 0.0f);
+    return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
-KEA_DEVI float key_float(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k); }
+KEA_DEVI float key_float(uint32_t k) { return __uint_as_float(k ^ ((uint32_t)((int)~k >> 31) | 0x80000000u)); }
 
-// The n-th largest of the lanes' values.
-KEA_DEVI float nth_largest(float v, int n, int lane) {
-    uint32_t key = float_key(v), top = 0;
-    for (int i = 0; i < n; ++i) {
-        top = __reduce_max_sync(0xFFFFFFFFu, key);
-        const uint32_t at = __ballot_sync(0xFFFFFFFFu, key == top);
-        if (lane == __ffs(at) - 1) key = 0;
+// An entry of a list: larger values first, equal ones by index, as one number to compare; 0: an empty place.
+KEA_DEVI uint64_t beam_entry(float v, int i) { return (uint64_t)float_key(v) << 32 | (uint32_t)~i; }
+KEA_DEVI float entry_value(uint64_t e) { return key_float((uint32_t)(e >> 32)); }
+KEA_DEVI int entry_index(uint64_t e) { return (int)~(uint32_t)e; }
+
+// The lanes' values in descending order.
+KEA_DEVI float sorted(float v, int lane) {
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            const float u = __shfl_xor_sync(0xFFFFFFFFu, v, j);
+            v = ((lane & k) == 0) == ((lane & j) == 0) ? fmaxf(v, u) : fminf(v, u);
+        }
+    return v;
+}
+
+// A warp's scratch: candidates on their way into its list, and the list while it is put together.
+struct __align__(16) BeamScratch {
+    uint64_t cand[64 + 2];
+    uint64_t list[kBeamMax + 2];
+};
+
+// Merges the first n <= 32 candidates of s.cand into the warp's sorted list: lane j < width holds the j-th entry, the
+// others nothing (0). Every lane counts what is ahead of its own entry and of its own candidate.
+KEA_DEVI void beam_merge(BeamScratch &s, int n, int width, int lane, uint64_t &list) {
+    const uint64_t mine = lane < n ? s.cand[lane] : 0;
+    s.list[lane] = list;
+    if (lane == 0) {   // the loops take two at a time
+        if (n & 1) s.cand[n] = 0;
+        if (width & 1) s.list[width] = 0;
     }
-    return key_float(top);
+    __syncwarp();
+    int place = lane, rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; j += 2) {
+        const ulonglong2 c = *reinterpret_cast<const ulonglong2 *>(s.cand + j);
+        place += (c.x > list) + (c.y > list);
+        rank += (c.x > mine) + (c.y > mine);
+    }
+#pragma unroll 4
+    for (int j = 0; j < width; j += 2) {
+        const ulonglong2 l = *reinterpret_cast<const ulonglong2 *>(s.list + j);
+        rank += (l.x > mine) + (l.y > mine);
+    }
+    __syncwarp();
+    if (lane < width && place < width) s.list[place] = list;
+    if (mine && rank < width) s.list[rank] = mine;
+    __syncwarp();
+    if (lane < width) list = s.list[lane];
+    __syncwarp();
 }
 
 struct BeamScan {
     float m = -INFINITY, off = 0.f;   // this lane's maximum and m log2 e (0 while there is none)
     float s = 0.f;                    // sum of 2^(x log2 e - off)
-    float lv = -INFINITY;             // the list
-    int li = kBeamNone;
+    uint32_t tiles = 0;               // key of the largest logit in this lane's group of tiles
+    float side = -INFINITY;           // this lane's value before the first or after the last vector
+    uint64_t list = 0;                // lane i: the i-th best logit
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -91,69 +117,82 @@ KEA_DEVI float exp2_approx(float v) {
     return r;
 }
 
-// E values per lane of one tile, x[e] at row index `index(e)` (ascending in the tile for ascending (e / EPV, lane, e %
-// EPV)); absent ones are -inf.
-template <typename T, int E, typename Index>
-KEA_DEVI void beam_tile(BeamScan &c, const float (&x)[E], const T *row, int width, int lane, Index index) {
-    float tm = x[0];
+// Adds E values per lane (absent ones -inf) to the lane's maximum and sum; returns their maximum (no NaN).
+template <int E>
+KEA_DEVI float beam_add(BeamScan &c, const float (&x)[E]) {
+    float tm = -INFINITY;
 #pragma unroll
-    for (int e = 1; e < E; ++e) tm = fmaxf(tm, x[e]);
+    for (int e = 0; e < E; ++e) tm = fmaxf(tm, x[e]);
     if (tm > c.m) {
         const float off = tm * kLog2e;
         c.s *= exp2_approx(c.off - off);   // 0 before the first finite logit
         c.m = tm;
         c.off = off;
     }
-    const float off = c.off;
-    float s0 = 0.f, s1 = 0.f;
+    if constexpr (E == 1) {
+        c.s += exp2_approx(fmaf(x[0], kLog2e, -c.off));
+    } else {
+        const uint64_t scale = pair_of(kLog2e, kLog2e), off = pair_of(-c.off, -c.off);
+        uint64_t sum = pair_of(0.f, 0.f);
 #pragma unroll
-    for (int e = 0; e < E; e += 2) {
-        s0 += exp2_approx(fmaf(x[e], kLog2e, -off));
-        if (e + 1 < E) s1 += exp2_approx(fmaf(x[e + 1], kLog2e, -off));
+        for (int e = 0; e < E; e += 2) {
+            float a, b;
+            unpair(fma2(pair_of(x[e], x[e + 1]), scale, off), a, b);
+            sum = add2(sum, pair_of(exp2_approx(a), exp2_approx(b)));
+        }
+        float a, b;
+        unpair(sum, a, b);
+        c.s += a + b;
     }
-    c.s += s0 + s1;
+    return tm;
+}
 
-    const float worst = __shfl_sync(0xFFFFFFFFu, c.lv, width - 1);
-    const uint32_t pass = __ballot_sync(0xFFFFFFFFu, tm > worst);
-    if (pass == 0) return;
-    const float bound = __popc(pass) >= width ? nth_largest(tm, width, lane) : -INFINITY;
-    uint32_t mask = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) mask |= (x[e] > worst && x[e] >= bound) ? 1u << e : 0u;
-    int entered = 0;
-    while (true) {
-        const uint32_t mine = mask ? (uint32_t)index(__ffs(mask) - 1) : 0xFFFFFFFFu;
-        const uint32_t next = __reduce_min_sync(0xFFFFFFFFu, mine);
-        if (next == 0xFFFFFFFFu) break;
-        const float v = to_float(row[next]);
-        if (mine == next) mask &= mask - 1;
-        const float lw = __shfl_sync(0xFFFFFFFFu, c.lv, width - 1);
-        const int iw = __shfl_sync(0xFFFFFFFFu, c.li, width - 1);
-        if (!beam_before(v, (int)next, lw, iw)) continue;
-        beam_insert(v, (int)next, lane, c.lv, c.li);
-        if (++entered == width) {   // the tile has filled the list: drop what is no longer above its end
-            entered = 0;
-            const float nw = __shfl_sync(0xFFFFFFFFu, c.lv, width - 1);
-            uint32_t keep = 0;
-#pragma unroll
-            for (int e = 0; e < E; ++e) keep |= (x[e] > nw) ? 1u << e : 0u;   // equal ones come later: behind
-            mask &= keep;
+// A warp's candidates on their way into its list.
+struct BeamGather {
+    BeamScratch &s;
+    uint64_t &list;
+    int width, lane, n = 0;
+    KEA_DEVI BeamGather(BeamScratch &scratch, uint64_t &l, int w, int ln) : s(scratch), list(l), width(w), lane(ln) {}
+    KEA_DEVI void flush(int k) {
+        __syncwarp();
+        beam_merge(s, k, width, lane, list);
+    }
+    KEA_DEVI void offer(bool good, uint64_t entry) {
+        const uint64_t end = __shfl_sync(0xFFFFFFFFu, list, width - 1);
+        good = good && entry > end;
+        const uint32_t votes = __ballot_sync(0xFFFFFFFFu, good);
+        if (votes == 0) return;
+        if (good) s.cand[n + __popc(votes & ((1u << lane) - 1u))] = entry;
+        n += __popc(votes);
+        if (n > 32) {
+            flush(32);
+            const uint64_t e = lane + 32 < n ? s.cand[32 + lane] : 0;
+            __syncwarp();
+            if (lane + 32 < n) s.cand[lane] = e;   // what is left moves down
+            __syncwarp();
+            n -= 32;
         }
     }
-}
+    KEA_DEVI void finish() {
+        if (n) flush(n);
+    }
+};
 
 template <typename T> struct BeamVec;   // a 16-byte vector of logits
 template <> struct BeamVec<float> {
     static constexpr int N = 4;
-    static KEA_DEVI void get(const float *p, float *v) {
-        const float4 w = *reinterpret_cast<const float4 *>(p);
-        v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+    static constexpr uint32_t kNone = 0xFF800000u;   // -inf
+    static KEA_DEVI void get(const uint4 &w, float *v) {
+        v[0] = __uint_as_float(w.x);
+        v[1] = __uint_as_float(w.y);
+        v[2] = __uint_as_float(w.z);
+        v[3] = __uint_as_float(w.w);
     }
 };
 template <typename T> struct BeamVec {
     static constexpr int N = 8;
-    static KEA_DEVI void get(const T *p, float *v) {
-        const uint4 w = *reinterpret_cast<const uint4 *>(p);
+    static constexpr uint32_t kNone = sizeof(T) == 2 && TypeCode<T>::value == KEA_TYPE_F16 ? 0xFC00FC00u : 0xFF80FF80u;
+    static KEA_DEVI void get(const uint4 &w, float *v) {
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -164,41 +203,83 @@ template <typename T> struct BeamVec {
     }
 };
 
-// One value per lane at lo + lane < hi.
+// A unit: logits lo .. hi - 1 of a row, as whole 16-byte vectors in tiles and the values before the first and after the
+// last vector (one per lane).
 template <typename T>
-KEA_DEVI void beam_edge(BeamScan &c, const T *row, int lo, int hi, int width, int lane) {
-    if (lo >= hi) return;
-    float x[1] = {-INFINITY};
-    if (lo + lane < hi) {
-        x[0] = to_float(row[lo + lane]);
+struct BeamUnit {
+    using Vec = BeamVec<T>;
+    static constexpr int N = Vec::N, V = sizeof(T) == 4 ? 4 : 2, E = N * V, TILE = 32 * V;   // vectors per tile
+    const T *row;
+    int lane, first, vecs, edge, group;   // group: tiles that share a lane's maximum
+    bool at_edge;
+    KEA_DEVI BeamUnit(const T *r, int lo, int hi, int l) : row(r), lane(l) {
+        const int head = min(hi - lo, (int)((16u - ((uint32_t)(reinterpret_cast<uintptr_t>(row + lo)) & 15u)) & 15u) / (int)sizeof(T));
+        first = lo + head;
+        vecs = (hi - first) / N;
+        const int last = first + vecs * N;
+        edge = lane < 16 ? lo + lane : last + lane - 16;   // at most 7 values on either side
+        at_edge = lane < 16 ? lane < head : edge < hi;
+        group = ((vecs + TILE - 1) / TILE + 31) / 32;
     }
-    beam_tile<T, 1>(c, x, row, width, lane, [&](int) { return lo + lane; });
-}
-
-// Logits lo .. hi - 1 of a row.
-template <typename T>
-KEA_DEVI void beam_scan(BeamScan &c, const T *row, int lo, int hi, int width, int lane) {
-    constexpr int N = BeamVec<T>::N, V = 4, E = N * V;
-    const int head = min(hi - lo, (int)((16u - ((uint32_t)(reinterpret_cast<uintptr_t>(row + lo)) & 15u)) & 15u) / (int)sizeof(T));
-    beam_edge(c, row, lo, lo + head, width, lane);
-    lo += head;
-    const int vecs = (hi - lo) / N;
-    for (int v0 = 0; v0 < vecs; v0 += 32 * V) {
-        float x[E];
+    KEA_DEVI void load(int v0, uint4 (&w)[V]) const {
+        const uint4 *p = reinterpret_cast<const uint4 *>(row + first);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int v = v0 + 32 * j + lane;
-            if (v < vecs) {
-                BeamVec<T>::get(row + lo + v * N, x + j * N);
-            } else {
+            w[j] = make_uint4(Vec::kNone, Vec::kNone, Vec::kNone, Vec::kNone);
+            if (v < vecs) w[j] = p[v];
+        }
+    }
+    KEA_DEVI void values(const uint4 (&w)[V], float (&x)[E]) const {
 #pragma unroll
-                for (int i = 0; i < N; ++i) x[j * N + i] = -INFINITY;
+        for (int j = 0; j < V; ++j) Vec::get(w[j], x + j * N);
+    }
+    KEA_DEVI void scan(BeamScan &c) const {
+        if (at_edge) c.side = to_float(row[edge]);
+        uint4 next[V];
+        load(0, next);
+        int left = group, owner = 0;
+        for (int v0 = 0; v0 < vecs; v0 += TILE) {
+            float x[E];
+            values(next, x);
+            load(v0 + TILE, next);
+            const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, float_key(beam_add(c, x)));
+            if (lane == owner) c.tiles = max(c.tiles, top);
+            if (--left == 0) {
+                left = group;
+                ++owner;
             }
         }
-        beam_tile<T, E>(c, x, row, width, lane, [&](int e) { return lo + (v0 + 32 * (e / N) + lane) * N + e % N; });
+        const float side[1] = {c.side};
+        beam_add(c, side);
     }
-    beam_edge(c, row, lo + vecs * N, hi, width, lane);
-}
+    // the values that reach `low`, into the list
+    KEA_DEVI void gather(BeamScan &c, float low, int width, BeamScratch &s) const {
+        BeamGather g(s, c.list, width, lane);
+        uint32_t todo = __ballot_sync(0xFFFFFFFFu, c.tiles >= float_key(low) && c.tiles > float_key(-INFINITY));
+        while (todo) {
+            const int v1 = __ffs(todo) * group * TILE;
+            todo &= todo - 1;
+            for (int v0 = v1 - group * TILE; v0 < min(v1, vecs); v0 += TILE) {
+                uint4 w[V];
+                load(v0, w);
+                float x[E];
+                values(w, x);
+                uint32_t mask = 0;   // this lane's values that do
+#pragma unroll
+                for (int e = 0; e < E; ++e) mask |= (x[e] >= low && x[e] > -INFINITY ? 1u : 0u) << e;
+                while (__any_sync(0xFFFFFFFFu, mask != 0)) {   // one of every lane at a time, hardly ever more than one
+                    const int e = mask ? __ffs(mask) - 1 : 0;
+                    const int i = first + (v0 + 32 * (e / N) + lane) * N + e % N;
+                    g.offer(mask != 0, mask ? beam_entry(to_float(row[i]), i) : 0);
+                    mask &= mask - 1;
+                }
+            }
+        }
+        g.offer(c.side >= low && c.side > -INFINITY, beam_entry(c.side, edge));
+        g.finish();
+    }
+};
 
 // log sum exp of logits lo .. hi - 1, the warp's lanes having scanned them; not a number: a logit of +inf.
 template <typename T>
@@ -225,81 +306,96 @@ KEA_DEVI double beam_log_sum(const BeamScan &c, const T *row, int lo, int hi, in
     return (double)m + (double)logf(s);
 }
 
-KEA_DEVI float ld_cluster_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
-
 KEA_DEVI double ld_cluster_f64(uint32_t addr) {
     double v;
     asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
     return v;
 }
+KEA_DEVI uint64_t ld_cluster_u64(uint32_t addr) {
+    uint64_t v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+    return v;
+}
 
-template <typename T>
-__global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(const BeamArgs a) {
-    constexpr int SLOTS = kBeamRounds * kBeamWarps;
-    __shared__ double ul[SLOTS];                                      // the units' log-sums
-    __shared__ float uv[SLOTS * kBeamMax];                            // and lists: [slot][width]
-    __shared__ int ui[SLOTS * kBeamMax];
-    __shared__ float lse[kBeamMax];                                   // first CTA: per hypothesis, NaN: offers nothing
-    __shared__ float wv[kBeamWarps * kBeamMax];                       // first CTA: the warps' merged lists
-    __shared__ int wi[kBeamWarps * kBeamMax];
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) beam_select_kernel(const BeamArgs a) {
+    __shared__ double ul[kBeamSlots];                  // the units' log-sums
+    __shared__ uint64_t ue[kBeamSlots * kBeamMax];     // and lists: [slot][width]
+    __shared__ float tops[2 * WARPS];                  // per warp: two of its largest lane maxima
+    __shared__ float score[kBeamMax], lse[kBeamMax];   // per hypothesis; lse not a number: it offers nothing
+    __shared__ bool over[kBeamMax];                    // it has ended
+    __shared__ BeamScratch scratch[WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int ctas = a.ctas, rank = (int)blockIdx.x % ctas, b = (int)blockIdx.x / ctas;   // a cluster is `ctas` consecutive CTAs
-    const int warps = ctas * kBeamWarps, K = a.beams, W = a.width;
+    const int warps = ctas * WARPS, K = a.beams, W = a.width;
+    BeamScratch &own = scratch[warp];
     grid_dependency_wait();
     grid_launch_dependents();
+    if (threadIdx.x < K) {
+        score[threadIdx.x] = a.scores[(long long)b * K + threadIdx.x];
+        over[threadIdx.x] = a.ended && a.ended[(long long)b * K + threadIdx.x];
+    }
+    __syncthreads();
 
+    // Several rounds only where every unit is a whole hypothesis; segments of one have one round, in which the warps of a
+    // CTA at the same hypothesis agree on its bound.
     for (int r = 0; r < a.rounds; ++r) {
-        const int unit = r * warps + rank * kBeamWarps + warp, slot = r * kBeamWarps + warp;
-        if (unit >= a.units) break;
-        const int k = unit / a.segs, seg = unit - k * a.segs;
+        const int unit = r * warps + rank * WARPS + warp, slot = r * WARPS + warp;
+        const bool some = unit < a.units;
+        const int k = some ? unit / a.segs : 0, seg = unit - k * a.segs;
+        const bool scans = some && !over[k];
+        const T *row = static_cast<const T *>(a.logits) + (long long)b * a.ld_clip + (long long)k * a.ld_beam;
+        const int per = (a.vocab + a.segs - 1) / a.segs, lo = scans ? min(a.vocab, seg * per) : 0, hi = scans ? min(a.vocab, lo + per) : 0;
         BeamScan c;
-        if (a.ended && a.ended[(long long)b * K + k]) {
-            if (seg == 0 && lane == 0) {
-                c.lv = 0.f;
-                c.li = a.end;
-            }
-        } else {
-            const T *row = static_cast<const T *>(a.logits) + (long long)b * a.ld_clip + (long long)k * a.ld_beam;
-            const int per = (a.vocab + a.segs - 1) / a.segs;
-            const int lo = min(a.vocab, seg * per);
-            const int hi = min(a.vocab, lo + per);
-            beam_scan(c, row, lo, hi, W, lane);
+        const BeamUnit<T> u(row, lo, hi, lane);
+        if (scans) {
+            u.scan(c);
             const double sum = beam_log_sum(c, row, lo, hi, lane);
             if (lane == 0) ul[slot] = sum;
+        } else if (some && seg == 0 && lane == 0) {
+            c.list = beam_entry(0.f, a.end);
         }
-        if (lane < W) {
-            uv[slot * W + lane] = c.lv;
-            ui[slot * W + lane] = c.li;
+        // `width` lanes of this warp reach low; of the n warps of this CTA at the hypothesis each has ceil(width / n) lanes
+        // that reach its own such value, so `width` lanes of them all reach the least of those
+        const float best = sorted(c.m, lane);
+        float low = __shfl_sync(0xFFFFFFFFu, best, W - 1);
+        if (a.segs > 1) {
+            const int w0 = max(0, warp - seg), n = max(1, min(WARPS, warp - seg + a.segs) - w0);   // its first warp, their number
+            const float few = __shfl_sync(0xFFFFFFFFu, best, (W + n - 1) / n - 1);
+            if (lane == 0) {
+                tops[warp] = low;
+                tops[WARPS + warp] = few;
+            }
+            __syncthreads();
+            const float other = lane < n ? tops[w0 + lane] : -INFINITY, least = lane < n ? tops[WARPS + w0 + lane] : INFINITY;
+            low = fmaxf(key_float(__reduce_max_sync(0xFFFFFFFFu, float_key(other))),
+                        key_float(__reduce_min_sync(0xFFFFFFFFu, float_key(least))));
         }
+        if (scans) u.gather(c, low, W, own);
+        if (some && lane < W) ue[slot * W + lane] = c.list;
     }
     if (ctas > 1) cluster_sync_all();
     else __syncthreads();
 
     if (rank == 0) {
-        // where unit u's results lie: CTA (u % warps) / 8, slot (u / warps) * 8 + u % 8
-        const auto at = [&](const void *base, int u, int words, int i) {
-            const int r = u / warps, w = u - r * warps;
-            return map_to_rank(smem_u32(base) + 4u * (uint32_t)((r * kBeamWarps + (w & (kBeamWarps - 1))) * words + i),
-                               (uint32_t)(w / kBeamWarps));
+        // where unit u's results lie: CTA (u % warps) / WARPS, slot (u / warps) * WARPS + u % WARPS
+        const auto at = [&](const void *base, int u, int each, int i) {
+            const int r = a.rounds == 1 ? 0 : u / warps, w = u - r * warps;
+            return map_to_rank(smem_u32(base) + 8u * (uint32_t)((r * WARPS + w % WARPS) * each + i), (uint32_t)(w / WARPS));
         };
-        for (int k = warp; k < K; k += kBeamWarps) {
-            // an ended hypothesis needs none
-            if (a.ended && a.ended[(long long)b * K + k]) {
-                if (lane == 0) lse[k] = 0.f;
-                continue;
-            }
+        for (int k = warp; k < K; k += WARPS) {
+            if (over[k]) continue;   // it needs none
             double top = -INFINITY;
-            for (int g = lane; g < a.segs; g += 32) top = fmax(top, ld_cluster_f64(at(ul, k * a.segs + g, 2, 0)));
+            for (int g = lane; g < a.segs; g += 32) top = fmax(top, ld_cluster_f64(at(ul, k * a.segs + g, 1, 0)));
+            if (a.segs > 1)
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+                for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            top = __shfl_sync(0xFFFFFFFFu, top, 0);
             float s = 0.f;   // a segment with a logit of +inf is not a number, and makes the whole so
-            for (int g = lane; g < a.segs; g += 32) s += expf((float)(ld_cluster_f64(at(ul, k * a.segs + g, 2, 0)) - top));
+            for (int g = lane; g < a.segs; g += 32) s += expf((float)(ld_cluster_f64(at(ul, k * a.segs + g, 1, 0)) - top));
+            if (a.segs > 1)
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+                for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
             if (lane == 0) {
                 // nothing is offered where it is infinite (no label left) or not a number
                 const float l = (float)(top + (double)logf(s));
@@ -307,76 +403,69 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(const BeamArg
             }
         }
         __syncthreads();
-        float lv = -INFINITY;
-        int li = kBeamNone;
-        const int entries = a.units * W;
-        for (int e0 = warp * 32; e0 < entries; e0 += kBeamThreads) {
-            const int e = e0 + lane;
-            float v = -INFINITY;
-            int i = kBeamNone;
-            if (e < entries) {
-                const int u = e / W, k = u / a.segs, p = e - u * W;
-                i = ld_cluster_s32(at(ui, u, W, p));
-                const float l = lse[k];
-                const float score = a.scores[(long long)b * K + k];
-                if (i != kBeamNone && l == l && fabsf(score) < INFINITY) {
-                    const float x = ld_cluster_f32(at(uv, u, W, p));
-                    v = (a.ended && a.ended[(long long)b * K + k]) ? score : __fadd_rn(__fsub_rn(x, l), score);
-                    i += k * a.vocab;
-                } else {
-                    i = kBeamNone;
+        // Merging in two levels: up to eight warps take the units' lists, whole lists to 32 lanes, then the first warp theirs.
+        uint64_t list = 0;
+        const auto enter = [&](uint64_t e) {   // 32 candidates: those that can enter, packed together
+            const bool good = e > __shfl_sync(0xFFFFFFFFu, list, W - 1);
+            const uint32_t pass = __ballot_sync(0xFFFFFFFFu, good);
+            if (pass == 0) return;
+            if (good) own.cand[__popc(pass & ((1u << lane) - 1u))] = e;
+            __syncwarp();
+            beam_merge(own, __popc(pass), W, lane, list);
+        };
+        const int each = 32 / W, mine = lane / W, q = lane - mine * W;   // lists per turn; this lane's list and place in it
+        const int takers = min(min(WARPS, 8), (a.units + each - 1) / each);
+        if (warp < takers)
+            for (int u0 = warp * each; u0 < a.units; u0 += takers * each) {
+                const int u = u0 + mine;
+                uint64_t e = 0;
+                if (mine < each && u < a.units) {
+                    const int k = a.segs == 1 ? u : u / a.segs;
+                    const float s = score[k], l = over[k] ? 0.f : lse[k];
+                    e = ld_cluster_u64(at(ue, u, W, q));
+                    if (e && l == l && fabsf(s) < INFINITY)
+                        e = beam_entry(over[k] ? s : __fadd_rn(__fsub_rn(entry_value(e), l), s), entry_index(e) + k * a.vocab);
+                    else
+                        e = 0;
                 }
+                enter(e);
             }
-            while (true) {
-                const float lw = __shfl_sync(0xFFFFFFFFu, lv, W - 1);
-                const int iw = __shfl_sync(0xFFFFFFFFu, li, W - 1);
-                const uint32_t pass = __ballot_sync(0xFFFFFFFFu, i != kBeamNone && beam_before(v, i, lw, iw));
-                if (pass == 0) break;
-                const int src = __ffs(pass) - 1;
-                beam_insert(__shfl_sync(0xFFFFFFFFu, v, src), __shfl_sync(0xFFFFFFFFu, i, src), lane, lv, li);
-                if (lane == src) i = kBeamNone;
-            }
+        if (takers > 1) {
+            __syncwarp();
+            own.list[lane] = list;
+            __syncthreads();
+            if (warp == 0)
+                for (int w = 1; w < takers; w += each) {
+                    const int from = w + mine;
+                    enter(mine < each && from < takers ? scratch[from].list[q] : 0);
+                }
         }
-        wv[warp * kBeamMax + lane] = lv;
-        wi[warp * kBeamMax + lane] = li;
-        __syncthreads();
         if (warp == 0) {
-            const int lists = min(kBeamWarps, (entries + 31) / 32);
-            for (int w = 1; w < lists; ++w) {
-                float v = wv[w * kBeamMax + lane];
-                int i = lane < W ? wi[w * kBeamMax + lane] : kBeamNone;
-                while (true) {
-                    const float lw = __shfl_sync(0xFFFFFFFFu, lv, W - 1);
-                    const int iw = __shfl_sync(0xFFFFFFFFu, li, W - 1);
-                    const uint32_t pass = __ballot_sync(0xFFFFFFFFu, i != kBeamNone && beam_before(v, i, lw, iw));
-                    if (pass == 0) break;
-                    const int src = __ffs(pass) - 1;
-                    beam_insert(__shfl_sync(0xFFFFFFFFu, v, src), __shfl_sync(0xFFFFFFFFu, i, src), lane, lv, li);
-                    if (lane == src) i = kBeamNone;
-                }
-            }
             // Places left over take what is not offered, by flat index: the lowest numbers that the list does not hold
             // (at most 31 are taken, so 63 numbers are enough).
-            const uint32_t some = __ballot_sync(0xFFFFFFFFu, lane < W && li != kBeamNone);
+            const uint32_t some = __ballot_sync(0xFFFFFFFFu, lane < W && list != 0);
+            float v = entry_value(list);
+            int i = entry_index(list);
             if (__popc(some) < W) {
                 uint32_t low = 0, high = 0;   // flat indices 0 .. 31 and 32 .. 63 that the list holds
-                if (lane < W && li < 32) low = 1u << li;
-                else if (lane < W && li < 64) high = 1u << (li - 32);
+                if (some >> lane & 1) {
+                    if (i < 32) low = 1u << i;
+                    else if (i < 64) high = 1u << (i - 32);
+                }
                 uint64_t open = ~(((uint64_t)__reduce_or_sync(0xFFFFFFFFu, high) << 32) | __reduce_or_sync(0xFFFFFFFFu, low));
-                for (int i = __popc(some); i < lane; ++i) open &= open - 1;
+                for (int j = __popc(some); j < lane; ++j) open &= open - 1;
                 if (lane < W && lane >= __popc(some)) {
-                    lv = -INFINITY;
-                    li = __ffsll((long long)open) - 1;
+                    v = -INFINITY;
+                    i = __ffsll((long long)open) - 1;
                 }
             }
             if (lane < W) {
                 const long long o = (long long)b * W + lane;
-                const int k = li / a.vocab, v = li - k * a.vocab;
-                a.out_scores[o] = lv;
+                const int k = i / a.vocab, label = i - k * a.vocab;
+                a.out_scores[o] = v;
                 a.parents[o] = k;
-                a.labels[o] = v;
-                if (a.out_ended)
-                    a.out_ended[o] = v == a.end || (a.ended && a.ended[(long long)b * K + k]) ? 1 : 0;
+                a.labels[o] = label;
+                if (a.out_ended) a.out_ended[o] = label == a.end || over[k] ? 1 : 0;
             }
         }
     }
