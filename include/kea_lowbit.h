@@ -352,7 +352,8 @@ enum {
     KEA_INT8_KERNEL_REG = 1,      /* warp-level MMAs on operands loaded straight into registers: few tokens */
     KEA_INT8_KERNEL_TILE64 = 2,   /* tcgen05, tiles of 128 tokens x 64 channels */
     KEA_INT8_KERNEL_TILE128 = 3,  /* tcgen05, 128 x 128 */
-    KEA_INT8_KERNEL_PAIR = 4      /* tcgen05 on CTA pairs, 256 x 256 */
+    KEA_INT8_KERNEL_PAIR = 4,     /* tcgen05 on CTA pairs, 256 x 256 */
+    KEA_INT8_KERNEL_SPLIT = 5     /* tcgen05, tiles of 128 x 64 shared by the CTAs of a cluster along K */
 };
 
 int kea_lowbit_int8_gemm(const KeaInt8Desc *desc, void *stream);

@@ -17,7 +17,7 @@ constexpr int kMaxDynSmem = 227 * 1024 - 1024;   // the kernels' static shared m
 
 int validate(const KeaInt8Desc *d) {
     if (!d || d->m < 0 || d->n < 1 || d->k < 1 || d->y_type < KEA_TYPE_F32 || d->y_type > KEA_TYPE_BF16 ||
-        (d->flags & ~(KEA_INT8_SILU | KEA_INT8_PDL)) || d->kernel < 0 || d->kernel > KEA_INT8_KERNEL_PAIR)
+        (d->flags & ~(KEA_INT8_SILU | KEA_INT8_PDL)) || d->kernel < 0 || d->kernel > KEA_INT8_KERNEL_SPLIT)
         return KEA_ERR_INVALID_VALUE;
     if (d->m == 0) return KEA_OK;
     if (!d->q || !d->qs || !d->w || !d->alpha || !d->y || d->ldq < d->k || d->ldw < d->k || d->ldy < d->n)
@@ -82,17 +82,19 @@ struct Launch {
 };
 
 // ---- register-operand kernel ---------------------------------------------------------------------------------------
-template <typename T, int CG, int RG, int D>
-cudaError_t launch_reg_as(const kea::Int8Args &a, int ks, bool pdl, void *stream) {
-    const int cn = 16 * CG * (kea::kI8RegWarps / ks);
-    const Launch l(dim3((unsigned)ceil_div(a.N, cn), (unsigned)ceil_div(a.M, 8 * RG), 1), kea::kI8RegThreads,
-                   (size_t)kea::i8reg_smem_bytes(ks, 8 * RG, cn), stream, pdl);
-    return cudaLaunchKernelEx(&l.cfg, kea::int8_gemm_reg_kernel<T, CG, RG, D>, a, ks);
+template <typename T, int RG, int D>
+cudaError_t launch_reg_as(const kea::Int8Args &a, int sms, bool pdl, void *stream) {
+    // eight channels per CTA as long as sixteen do not give every SM one
+    const bool half = ceil_div(a.N, 16) * ceil_div(a.M, 8 * RG) < sms;
+    const Launch l(dim3((unsigned)ceil_div(a.N, half ? 8 : 16), (unsigned)ceil_div(a.M, 8 * RG), 1), kea::kI8RegThreads, 0, stream, pdl);
+    return half ? cudaLaunchKernelEx(&l.cfg, kea::int8_gemm_reg_kernel<T, RG, D, true>, a)
+                : cudaLaunchKernelEx(&l.cfg, kea::int8_gemm_reg_kernel<T, RG, D, false>, a);
 }
 
 template <typename T>
 cudaError_t launch_reg(const kea::Int8Args &a, int sms, bool pdl, void *stream) {
-    return launch_reg_as<T, 2, 4, 2>(a, a.K >= 512 ? 4 : 1, pdl, stream);
+    return a.M <= 8    ? launch_reg_as<T, 1, 8>(a, sms, pdl, stream)
+           : a.M <= 16 ? launch_reg_as<T, 2, 6>(a, sms, pdl, stream) : launch_reg_as<T, 4, 4>(a, sms, pdl, stream);
 }
 
 // ---- tcgen05 kernels -----------------------------------------------------------------------------------------------
@@ -152,9 +154,43 @@ cudaError_t launch_tile_as(const kea_host::Device &dev, const kea::Int8Args &a, 
     return cudaLaunchKernelEx(&l.cfg, kea::int8_gemm_tile_kernel<T, SILU, false, CTAS, BN>, qmap, wmap, ymap, p);
 }
 
+// How many CTAs share a 128 x 64 tile: as many as find an SM of their own, each with two blocks of K at least.
+int tile_splits(int m, int n, int k, int sms) {
+    const long long tiles = (long long)ceil_div(m, 128) * ceil_div(n, 64);
+    const int kbs = ceil_div(k, kea::kI8K);
+    int s = 1;
+    while (s < 8 && 2 * s * tiles <= sms && 4 * s <= kbs) s *= 2;
+    return ceil_div(kbs, ceil_div(kbs, s)) == s ? s : 1;   // (a power of two) no slice without work
+}
+
+template <typename T, bool SILU>
+cudaError_t launch_split(const kea_host::Device &dev, const kea::Int8Args &a, int splits, bool pdl, void *stream) {
+    using Tile = kea::Int8Tile<1, 64>;
+    kea::Int8TileArgs p{};
+    p.a = a;
+    p.n_tiles = ceil_div(a.N, 64);
+    p.tiles = p.n_tiles * ceil_div(a.M, 128);
+    p.kbs = ceil_div(a.K, kea::kI8K);
+    p.splits = splits;
+    p.per_split = ceil_div(p.kbs, splits);
+    // three stages at most: two CTAs per SM, so that 16 clusters of 8 run at once (one per SM leaves room for 15: a second
+    // wave, 13.4 instead of 10.3 us at 128 x 1024 x 4096)
+    p.stages = std::min(3, stages_for<1, 64>(p.per_split, 1));
+    CUtensorMap qmap, wmap, ymap{};
+    if (!map_codes(dev, &qmap, a.q, a.ldq, a.M, a.K, 128) || !map_codes(dev, &wmap, a.w, a.ldw, a.N, a.K, 64)) return cudaErrorInvalidValue;
+    p.tma_store = aligned(a.y, 16) && (a.ldy * (long long)sizeof(T)) % 16 == 0;   // here: rows take 16-byte stores
+    const Launch l(dim3((unsigned)(p.tiles * splits), 1, 1), Tile::THREADS, Tile::smem(p.stages), stream, pdl, splits);
+    return cudaLaunchKernelEx(&l.cfg, kea::int8_gemm_tile_kernel<T, SILU, false, 1, 64, true>, qmap, wmap, ymap, p);
+}
+
 template <typename T>
 cudaError_t launch_typed(const kea_host::Device &dev, const kea::Int8Args &a, int kernel, bool pdl, void *stream) {
     switch (kernel) {
+        case KEA_INT8_KERNEL_SPLIT: {
+            const int splits = tile_splits(a.M, a.N, a.K, dev.sms);
+            if (splits > 1) return a.silu ? launch_split<T, true>(dev, a, splits, pdl, stream) : launch_split<T, false>(dev, a, splits, pdl, stream);
+            [[fallthrough]];   // nothing to split: the same tiles, one CTA each
+        }
         case KEA_INT8_KERNEL_TILE64:
             return a.silu ? launch_tile_as<T, true, 1, 64>(dev, a, pdl, stream) : launch_tile_as<T, false, 1, 64>(dev, a, pdl, stream);
         case KEA_INT8_KERNEL_TILE128:
@@ -165,11 +201,37 @@ cudaError_t launch_typed(const kea_host::Device &dev, const kea::Int8Args &a, in
     }
 }
 
+// Which kernel, by the microseconds each is expected to take. A launch of the tile kernels lasts as long as its waves of
+// tiles: a fixed part, then per wave a part that grows with K (a CTA's MMAs are issue-paced, about 100 clocks per 32
+// columns of K). Fitted to launches back to back on a B200, measured / expected at M x N x K, us:
+//   register operands  32 x 4096 x 1024  4.4 / 4.4   128 x 1024 x 4096 11.1 / 11.6   512 x 640 x 640   9.3 / 9.8
+//   128 x 64 tiles    128 x 2048 x 256   4.1 / 3.9  1024 x 1024 x 1024  6.2 / 5.7   1024 x 4096 x 1024 14.2 / 14.1
+//   split tiles       128 x 1024 x 4096 10.3 / 10.1  256 x 1024 x 4096  9.1 / 10.1   512 x 1024 x 4096 12.6 / 12.0
+//   128 x 128 tiles   512 x 4096 x 1024  7.5 / 6.3  1024 x 4096 x 1024 10.7 / 9.5   1024 x 4096 x 4096 25.0 / 23.4
+//   pairs            1024 x 4096 x 1024 10.1 / 8.6  2048 x 4096 x 1024 13.3 / 11.9  1024 x 4096 x 4096 18.0 / 16.4
 int choose(const kea::Int8Args &a, int sms) {
-    if (a.M <= 64) return KEA_INT8_KERNEL_REG;
-    if ((long long)ceil_div(a.M, 256) * ceil_div(a.N, 256) >= sms / 2) return KEA_INT8_KERNEL_PAIR;
-    if ((long long)ceil_div(a.M, 128) * ceil_div(a.N, 128) >= sms / 2) return KEA_INT8_KERNEL_TILE128;
-    return KEA_INT8_KERNEL_TILE64;
+    const auto tiles = [&](int rows, int cols) { return (long long)ceil_div(a.M, rows) * ceil_div(a.N, cols); };
+    const double k = a.K;
+    const size_t size = a.y_type == KEA_TYPE_F32 ? 4 : 2;
+    // rows that TMA cannot store, or a skip connection it cannot be read beside, go out value by value
+    const double odd = !aligned(a.y, 16) || (a.ldy * size) % 16 || (a.res && ((a.ld_res * size) % 16 || (a.N * size) % 16)) ? 2.0 : 0.0;
+    const auto waves = [&](long long n, int at_once) { return (double)((n + at_once - 1) / at_once); };
+    int best = KEA_INT8_KERNEL_TILE64;
+    double least = 3.3 + 0.00235 * k + odd + (waves(tiles(128, 64), sms) - 1) * (0.6 + 0.00215 * k);
+    const auto offer = [&](int kernel, double us) {
+        if (us < least) {
+            least = us;
+            best = kernel;
+        }
+    };
+    if (a.M <= 4096)
+        offer(KEA_INT8_KERNEL_REG, std::max(2.9, 0.8 + 0.0047 * (double)tiles(a.M <= 16 ? 8 : 32, 16) * (a.M <= 16 ? 0.5 : 1.0) *
+                                                           (ceil_div(a.K, 512) + 1)));
+    const int s = tile_splits(a.M, a.N, a.K, sms);
+    if (s > 1) offer(KEA_INT8_KERNEL_SPLIT, 6.4 + 0.00245 * k / s + 0.3 * s);
+    offer(KEA_INT8_KERNEL_TILE128, 3.9 + 0.00235 * k + odd + (waves(tiles(128, 128), sms) - 1) * (0.9 + 0.0022 * k));
+    offer(KEA_INT8_KERNEL_PAIR, 6.0 + 0.00255 * k + odd + (waves(tiles(256, 256), sms / 2) - 1) * (1.05 + 0.0022 * k));
+    return best;
 }
 
 template <typename T, bool SILU, bool EXTRA>
@@ -179,7 +241,8 @@ bool attributes() {
     };
     return set((const void *)kea::int8_gemm_tile_kernel<T, SILU, EXTRA, 1, 64>) &&
            set((const void *)kea::int8_gemm_tile_kernel<T, SILU, EXTRA, 1, 128>) &&
-           set((const void *)kea::int8_gemm_tile_kernel<T, SILU, EXTRA, 2, 256>);
+           set((const void *)kea::int8_gemm_tile_kernel<T, SILU, EXTRA, 2, 256>) &&
+           (EXTRA || set((const void *)kea::int8_gemm_tile_kernel<T, SILU, false, 1, 64, true>));
 }
 template <typename T>
 bool attributes() {

@@ -10,8 +10,9 @@
 // MMAs): lane (g, t) (g = lane / 4, t = lane % 4) holds bytes 16 t .. 16 t + 15 of rows g and g + 8 of its 16 channels and of
 // token row g; bytes 0-3 / 4-7 of a 16-byte group are the first MMA's two k registers, 8-11 / 12-15 the second's.
 //
-// Work split. A CTA = 8 warps owns CN channels x 8 RG tokens; the warps are KS slices of K x (8 / KS) groups of 16 CG
-// channels. The slices' INT32 sums meet in shared memory and are added in slice order (exact), then finished.
+// Work split. A CTA owns 16 channels (8 where that leaves SMs without one: the MMA's upper rows stay empty) x 8 RG tokens; its
+// 8 warps are slices of K, whose INT32 sums meet in shared memory, are added in slice order (exact) and finished. A warp
+// keeps D steps in flight, so with K <= 512 D its whole share is asked for at once.
 // Weights do not depend on the previous kernel of the stream: the first loads are issued before griddepcontrol.wait.
 #pragma once
 
@@ -20,8 +21,6 @@
 namespace kea {
 
 constexpr int kI8RegThreads = 256, kI8RegWarps = 8, kI8RegPad = 4;
-
-__host__ __device__ inline int i8reg_smem_bytes(int ks, int rows, int cn) { return ks * rows * (cn + kI8RegPad) * 4; }
 
 KEA_DEVI void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -43,100 +42,89 @@ KEA_DEVI uint4 load_codes(const int8_t *row, int k, int K) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <typename T, int CG, int RG, int D>
-__global__ void __launch_bounds__(kI8RegThreads, 2) int8_gemm_reg_kernel(const Int8Args a, int KS) {
-    extern __shared__ __align__(16) int rsm[];
+template <typename T, int RG, int D, bool HALF>
+__global__ void __launch_bounds__(kI8RegThreads, 2) int8_gemm_reg_kernel(const Int8Args a) {
+    constexpr int R = 8 * RG, H = HALF ? 1 : 2, CN = 8 * H, KS = kI8RegWarps, LD = 16 + kI8RegPad;
+    __shared__ int part[KS * R * LD];   // [slice][token][channel]
     grid_launch_dependents();
-    constexpr int R = 8 * RG;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    const int CW = kI8RegWarps / KS, kw = warp % KS, cw = warp / KS;
-    const int CN = 16 * CG * CW;
     const int c0 = blockIdx.x * CN, m0 = blockIdx.y * R;
     const int steps = (a.K + 63) / 64, per = (steps + KS - 1) / KS;
-    const int s0 = min(steps, kw * per), s1 = min(steps, s0 + per);
+    const int s0 = min(steps, warp * per), s1 = min(steps, s0 + per);
 
-    const int8_t *wrow[CG][2], *qrow[RG];
+    const int8_t *wrow[H], *qrow[RG];
 #pragma unroll
-    for (int c = 0; c < CG; ++c)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int n = c0 + 16 * (cw * CG + c) + g + 8 * h;
-            wrow[c][h] = n < a.N ? a.w + (long long)n * a.ldw : nullptr;
-        }
+    for (int h = 0; h < H; ++h) {
+        const int n = c0 + g + 8 * h;
+        wrow[h] = n < a.N ? a.w + (long long)n * a.ldw : nullptr;
+    }
 #pragma unroll
     for (int r = 0; r < RG; ++r) {
         const int m = m0 + 8 * r + g;
         qrow[r] = m < a.M ? a.q + (long long)m * a.ldq : nullptr;
     }
 
-    uint4 wr[D][CG][2], br[D][RG];
+    uint4 wr[D][H], br[D][RG];
 #pragma unroll
     for (int d = 0; d < D; ++d)
 #pragma unroll
-        for (int c = 0; c < CG; ++c)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                wr[d][c][h] = load_codes<true>(wrow[c][h], s0 + d < s1 ? 64 * (s0 + d) + 16 * t : a.K, a.K);
+        for (int h = 0; h < H; ++h) wr[d][h] = load_codes<true>(wrow[h], s0 + d < s1 ? 64 * (s0 + d) + 16 * t : a.K, a.K);
     grid_dependency_wait();
 #pragma unroll
     for (int d = 0; d < D; ++d)
 #pragma unroll
-        for (int r = 0; r < RG; ++r)
-            br[d][r] = load_codes<false>(qrow[r], s0 + d < s1 ? 64 * (s0 + d) + 16 * t : a.K, a.K);
+        for (int r = 0; r < RG; ++r) br[d][r] = load_codes<false>(qrow[r], s0 + d < s1 ? 64 * (s0 + d) + 16 * t : a.K, a.K);
 
-    int acc[CG][RG][4];
+    int acc[RG][4];
 #pragma unroll
-    for (int c = 0; c < CG; ++c)
+    for (int r = 0; r < RG; ++r)
 #pragma unroll
-        for (int r = 0; r < RG; ++r)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[c][r][i] = 0;
+        for (int i = 0; i < 4; ++i) acc[r][i] = 0;
 
     for (int base = s0; base < s1; base += D) {
 #pragma unroll
         for (int d = 0; d < D; ++d) {
             const int s = base + d;
             if (s >= s1) break;
+            const uint4 lo = wr[d][0], hi = HALF ? make_uint4(0u, 0u, 0u, 0u) : wr[d][H - 1];
 #pragma unroll
-            for (int c = 0; c < CG; ++c)
+            for (int r = 0; r < RG; ++r) {
+                mma_s8(acc[r], lo.x, hi.x, lo.y, hi.y, br[d][r].x, br[d][r].y);
+                mma_s8(acc[r], lo.z, hi.z, lo.w, hi.w, br[d][r].z, br[d][r].w);
+            }
+            if (base + D < s1) {   // this slot's next step
+                const int k = s + D < s1 ? 64 * (s + D) + 16 * t : a.K;
 #pragma unroll
-                for (int r = 0; r < RG; ++r) {
-                    mma_s8(acc[c][r], wr[d][c][0].x, wr[d][c][1].x, wr[d][c][0].y, wr[d][c][1].y, br[d][r].x, br[d][r].y);
-                    mma_s8(acc[c][r], wr[d][c][0].z, wr[d][c][1].z, wr[d][c][0].w, wr[d][c][1].w, br[d][r].z, br[d][r].w);
-                }
-            const int k = s + D < s1 ? 64 * (s + D) + 16 * t : a.K;   // this slot's next step
+                for (int h = 0; h < H; ++h) wr[d][h] = load_codes<true>(wrow[h], k, a.K);
 #pragma unroll
-            for (int c = 0; c < CG; ++c)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) wr[d][c][h] = load_codes<true>(wrow[c][h], k, a.K);
-#pragma unroll
-            for (int r = 0; r < RG; ++r) br[d][r] = load_codes<false>(qrow[r], k, a.K);
+                for (int r = 0; r < RG; ++r) br[d][r] = load_codes<false>(qrow[r], k, a.K);
+            }
         }
     }
 
     // the D fragment: channels g / g + 8, token rows 2 t / 2 t + 1
-    const int ld = CN + kI8RegPad;
-    int *part = rsm + kw * R * ld;
+    int *own = part + warp * R * LD;
 #pragma unroll
-    for (int c = 0; c < CG; ++c)
-#pragma unroll
-        for (int r = 0; r < RG; ++r) {
-            const int ch = 16 * (cw * CG + c) + g, row = 8 * r + 2 * t;
-            part[row * ld + ch] = acc[c][r][0];
-            part[(row + 1) * ld + ch] = acc[c][r][1];
-            part[row * ld + ch + 8] = acc[c][r][2];
-            part[(row + 1) * ld + ch + 8] = acc[c][r][3];
+    for (int r = 0; r < RG; ++r) {
+        const int row = 8 * r + 2 * t;
+        own[row * LD + g] = acc[r][0];
+        own[(row + 1) * LD + g] = acc[r][1];
+        if (!HALF) {
+            own[row * LD + g + 8] = acc[r][2];
+            own[(row + 1) * LD + g + 8] = acc[r][3];
         }
+    }
     __syncthreads();
     for (int i = threadIdx.x; i < R * CN; i += kI8RegThreads) {
-        const int row = i / CN, ch = i - row * CN, m = m0 + row, n = c0 + ch;
+        const int row = i / CN, ch = i % CN, m = m0 + row, n = c0 + ch;
         if (m >= a.M || n >= a.N) continue;
-        int v = 0;
-        for (int w = 0; w < KS; ++w) v += rsm[(w * R + row) * ld + ch];
-        if (a.acc) a.acc[(long long)m * a.ld_acc + n] = v;
         const uint64_t s = pair_of(a.qs[m], 0.f), alpha = pair_of(__ldg(a.alpha + n), 0.f);
         const uint64_t bias = pair_of(a.bias ? __ldg(a.bias + n) : kI8NoBias, 0.f);
+        int v = 0;
+#pragma unroll
+        for (int w = 0; w < KS; ++w) v += part[(w * R + row) * LD + ch];
+        if (a.acc) a.acc[(long long)m * a.ld_acc + n] = v;
         float y, unused;
         unpair(a.silu ? int8_values<true>(v, 0, s, alpha, bias) : int8_values<false>(v, 0, s, alpha, bias), y, unused);
         int8_store<T>(a, m, n, y);

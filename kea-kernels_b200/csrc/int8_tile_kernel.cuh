@@ -11,6 +11,11 @@
 // 32 tensor-memory lanes it may and 64 columns: TMEM -> scales, bias, SiLU, skip connection -> boxes of 32 rows
 // x 128 bytes staged in shared memory (128-byte swizzle) -> TMA stores, or row-wise stores where the output's rows are
 // not 16-byte aligned. Every wait is bounded; one that runs out is reported in the error word and the kernel ends.
+//
+// SPLIT (single CTAs, 64 channels): few tiles and a long K. A cluster of 2, 4 or 8 CTAs shares a tile, each taking a slice of
+// K (a CTA issues about 100 clocks per MMA whatever its N, so the length of K, not its products, sets a launch's time);
+// each sends every other the INT32 sums of the channels that one finishes (distributed shared memory), and after a cluster
+// barrier adds the slices' sums of its own, exactly.
 #pragma once
 
 #include "int8_epilogue.cuh"
@@ -36,6 +41,7 @@ struct Int8TileArgs {
     Int8Args a;
     int n_tiles, tiles, kbs, stages;
     int tma_store, res_vec;
+    int splits, per_split;    // CTAs that share a tile, blocks of K each takes (SPLIT)
 };
 
 KEA_DEVI void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
@@ -207,10 +213,87 @@ KEA_DEVI void int8_epilogue_tile(const Int8TileArgs &p, const CUtensorMap *ymap,
 template <> KEA_DEVI uint32_t pack2<float>(float, float) { return 0u; }
 template <> KEA_DEVI float2 unpack2<float>(uint32_t) { return make_float2(0.f, 0.f); }
 
-template <typename T, bool SILU, bool EXTRA, int CTAS, int BN>
+// Split tiles: this warp's 32 rows of every rank's channels to their owners' receive space, [source][128 rows][cw].
+KEA_DEVI void int8_send_sums(uint32_t taddr, uint32_t recv, int cw, int splits, uint32_t rank, int quad) {
+    const int row = quad * 32 + (int)(threadIdx.x & 31);
+#pragma unroll 1
+    for (int c = 0; c < 64; c += 8) {
+        uint32_t v[8];
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                     : "r"(taddr + (uint32_t)c)
+                     : "memory");
+        tmem_wait_ld();
+        asm volatile("" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]) : : "memory");
+        const int owner = c / cw;
+        const uint32_t at = map_to_rank(recv + (uint32_t)(((int)rank * 128 + row) * cw + c - owner * cw) * 4u, (uint32_t)owner);
+        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + 16u), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+    }
+}
+
+// The slices' sums of this CTA's cw channels, added and finished: eight channels of a row per lane at a time.
+template <typename T, bool SILU>
+KEA_DEVI void int8_finish_split(const Int8TileArgs &p, uint32_t recv, uint32_t consts, int cw, uint32_t rank, int quad, int m0, int n0,
+                                uint64_t sq) {
+    const Int8Args &a = p.a;
+    const int row = quad * 32 + (int)(threadIdx.x & 31), m = m0 + row;
+    if (m >= a.M) return;
+#pragma unroll 1
+    for (int c = 0; c < cw; c += 8) {
+        const int col = (int)rank * cw + c, n = n0 + col;   // in the tile, in the output
+        if (n >= a.N) break;
+        int v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        for (int s = 0; s < p.splits; ++s)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint4 u = ld_shared16(recv + (uint32_t)((s * 128 + row) * cw + c + 4 * h) * 4u);
+                v[4 * h] += (int)u.x;
+                v[4 * h + 1] += (int)u.y;
+                v[4 * h + 2] += (int)u.z;
+                v[4 * h + 3] += (int)u.w;
+            }
+        float f[8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const ulonglong2 al = ld_shared_pairs(consts + (uint32_t)(col + 4 * h) * 4u);
+            const ulonglong2 bi = ld_shared_pairs(consts + (uint32_t)(64 + col + 4 * h) * 4u);
+            unpair(int8_values<SILU>(v[4 * h], v[4 * h + 1], sq, al.x, bi.x), f[4 * h], f[4 * h + 1]);
+            unpair(int8_values<SILU>(v[4 * h + 2], v[4 * h + 3], sq, al.y, bi.y), f[4 * h + 2], f[4 * h + 3]);
+        }
+        const bool whole = n + 8 <= a.N;
+        if (a.res) {
+            const T *r = static_cast<const T *>(a.res) + (long long)m * a.ld_res + n;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (n + j < a.N) f[j] = __fadd_rn(to_float(r[j]), __fmul_rn(a.res_scale, f[j]));
+        }
+        if (a.acc) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (n + j < a.N) a.acc[(long long)m * a.ld_acc + n + j] = v[j];
+        }
+        T *y = static_cast<T *>(a.y) + (long long)m * a.ldy + n;
+        if (whole && p.tma_store) {   // rows 16-byte aligned
+            if constexpr (sizeof(T) == 4) {
+                reinterpret_cast<float4 *>(y)[0] = make_float4(f[0], f[1], f[2], f[3]);
+                reinterpret_cast<float4 *>(y)[1] = make_float4(f[4], f[5], f[6], f[7]);
+            } else {
+                *reinterpret_cast<uint4 *>(y) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (n + j < a.N) y[j] = from_float<T>(f[j]);
+        }
+    }
+}
+
+template <typename T, bool SILU, bool EXTRA, int CTAS, int BN, bool SPLIT = false>
 __global__ void __launch_bounds__(Int8Tile<CTAS, BN>::THREADS, 1)
 int8_gemm_tile_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap wmap,
                       const __grid_constant__ CUtensorMap ymap, const Int8TileArgs p) {
+    static_assert(!SPLIT || (CTAS == 1 && BN == 64), "split tiles are single CTAs' of 64 channels");
     using Tile = Int8Tile<CTAS, BN>;
     extern __shared__ uint8_t dyn_smem[];
     __shared__ __align__(8) uint64_t bar_full[kI8MaxStages];    // (pairs: in the even CTA) both operands of a stage landed
@@ -221,8 +304,10 @@ int8_gemm_tile_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     __shared__ uint32_t tmem_slot;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = CTAS == 2 ? cluster_ctarank() : 0u;
-    const int worker = (int)blockIdx.x / CTAS, workers = (int)gridDim.x / CTAS;
+    // a pair's CTA, or the slice of K a split tile's CTA takes
+    const uint32_t rank = CTAS == 2 ? cluster_ctarank() : 0u, slice = SPLIT ? cluster_ctarank() : 0u;
+    const int worker = (int)blockIdx.x / (SPLIT ? p.splits : CTAS), workers = (int)gridDim.x / (SPLIT ? p.splits : CTAS);
+    const int kb0 = SPLIT ? (int)slice * p.per_split : 0, kb1 = SPLIT ? min(p.kbs, kb0 + p.per_split) : p.kbs;
     const uint32_t base = (smem_u32(dyn_smem) + 1023u) & ~1023u;
     const int S = p.stages;
     const uint32_t A0 = base, B0 = base + (uint32_t)S * kI8Half;
@@ -254,7 +339,7 @@ int8_gemm_tile_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         }
     }
     tc_fence_before();
-    if constexpr (CTAS == 2) cluster_sync_all();
+    if constexpr (CTAS == 2 || SPLIT) cluster_sync_all();
     else __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
@@ -268,7 +353,7 @@ int8_gemm_tile_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             for (int tile = worker; tile < p.tiles && ok; tile += workers) {
                 const int mt = tile / p.n_tiles, nt = tile - mt * p.n_tiles;
                 const int t0 = mt * 128 * CTAS + (int)rank * 128, n0 = nt * BN + (int)rank * (BN / CTAS);
-                for (int kb = 0; kb < p.kbs; ++kb) {
+                for (int kb = kb0; kb < kb1; ++kb) {
                     if (issued >= S && !mbar_wait(smem_u32(&bar_empty[s]), ph ^ 1u, kOpWaitBudget)) {
                         ok = false;
                         break;
@@ -315,7 +400,7 @@ int8_gemm_tile_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 }
                 tc_fence_after();
                 const uint32_t dcol = tmem + (uint32_t)buf * BN;
-                for (int kb = 0; kb < p.kbs; ++kb) {
+                for (int kb = kb0; kb < kb1; ++kb) {
                     const bool ready = CTAS == 2 ? mbar_wait_cluster(smem_u32(&bar_full[s]), ph, kOpWaitBudget)
                                                  : mbar_wait(smem_u32(&bar_full[s]), ph, kOpWaitBudget);
                     if (!__all_sync(0xFFFFFFFFu, ready)) {
@@ -328,7 +413,7 @@ int8_gemm_tile_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                     if (elect_one()) {
 #pragma unroll
                         for (int kk = 0; kk < kI8K / 32; ++kk) {   // K = 32 per MMA: + 32 bytes = 2 descriptor units
-                            const uint32_t more = (kb > 0 || kk > 0) ? 1u : 0u;
+                            const uint32_t more = (kb > kb0 || kk > 0) ? 1u : 0u;
                             if constexpr (CTAS == 2) mma_i8_pair(dcol, ad + (uint64_t)(2 * kk), bd + (uint64_t)(2 * kk), idesc, more);
                             else mma_i8(dcol, ad + (uint64_t)(2 * kk), bd + (uint64_t)(2 * kk), idesc, more);
                         }
@@ -357,6 +442,25 @@ int8_gemm_tile_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             __syncwarp();
             mbar_wait(smem_u32(&bar_drain), 0u, kOpWaitBudget);
             __syncwarp();
+        }
+    } else if constexpr (SPLIT) {   // one tile per cluster
+        const int ew = warp - 2, quad = warp & 3, mt = worker / p.n_tiles, m0 = mt * 128, n0 = (worker - mt * p.n_tiles) * BN;
+        const uint32_t consts = CONST0 + (uint32_t)(ew * Tile::CW) * 8u;
+#pragma unroll
+        for (int i = 0; i < Tile::CW; i += 32) {
+            const int n = n0 + i + lane;
+            const float al = n < p.a.N ? __ldg(p.a.alpha + n) : 0.f;
+            const float bi = p.a.bias && n < p.a.N ? __ldg(p.a.bias + n) : kI8NoBias;
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(consts + (uint32_t)(i + lane) * 4u), "f"(al) : "memory");
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(consts + (uint32_t)(Tile::CW + i + lane) * 4u), "f"(bi) : "memory");
+        }
+        __syncwarp();
+        const bool done = mbar_wait_sleep(smem_u32(&bar_acc_full[0]), 0u, kOpWaitBudget, 64);
+        if (__all_sync(0xFFFFFFFFu, done)) {
+            tc_fence_after();
+            int8_send_sums(tmem + ((uint32_t)(quad * 32) << 16), STG0, BN / p.splits, p.splits, slice, quad);
+        } else if (lane == 0) {
+            report_error(p.a.err, KEA_DEVERR_TIMEOUT);
         }
     } else {
         const int ew = warp - 2, quad = warp & 3, part = ew >> 2;
@@ -404,8 +508,16 @@ int8_gemm_tile_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
 
     grid_launch_dependents();
     tc_fence_before();
-    if constexpr (CTAS == 2) cluster_sync_relaxed_paths();
+    if constexpr (CTAS == 2 || SPLIT) cluster_sync_relaxed_paths();
     else __syncthreads();
+    if constexpr (SPLIT) {
+        if (warp >= 2) {   // every slice's sums have arrived
+            const int ew = warp - 2, quad = warp & 3, mt = worker / p.n_tiles, m0 = mt * 128, n0 = (worker - mt * p.n_tiles) * BN;
+            const int m = m0 + quad * 32 + lane;
+            const float s = m < p.a.M ? p.a.qs[m] : 0.f;
+            int8_finish_split<T, SILU>(p, STG0, CONST0 + (uint32_t)(ew * Tile::CW) * 8u, BN / p.splits, slice, quad, m0, n0, pair_of(s, s));
+        }
+    }
     if (warp == 1) {
         tc_fence_after();
         if constexpr (CTAS == 2) tmem_dealloc_pair(tmem, kCols);

@@ -31,7 +31,7 @@ EXPORTS = ("kea_lowbit_gemm", "kea_lowbit_gemm_noalloc", "kea_lowbit_choose_conf
            "kea_lowbit_status_string", "kea_lowbit_version",
            "kea_lowbit_int8_gemm", "kea_lowbit_residual_norm", "kea_lowbit_beam_select", "kea_lowbit_beam_reorder")
 CONV_PDL, CONV_QUANT_SILU = 1, 2
-INT8_KERNEL_REG, INT8_KERNEL_TILE64, INT8_KERNEL_TILE128, INT8_KERNEL_PAIR = 1, 2, 3, 4
+INT8_KERNEL_REG, INT8_KERNEL_TILE64, INT8_KERNEL_TILE128, INT8_KERNEL_PAIR, INT8_KERNEL_SPLIT = 1, 2, 3, 4, 5
 
 
 class GemmDesc(ctypes.Structure):

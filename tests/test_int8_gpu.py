@@ -14,7 +14,8 @@ from kea_kernels import _lib, lowbit
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
-KERNELS = [0, _lib.INT8_KERNEL_REG, _lib.INT8_KERNEL_TILE64, _lib.INT8_KERNEL_TILE128, _lib.INT8_KERNEL_PAIR]
+KERNELS = [0, _lib.INT8_KERNEL_REG, _lib.INT8_KERNEL_TILE64, _lib.INT8_KERNEL_TILE128, _lib.INT8_KERNEL_PAIR,
+           _lib.INT8_KERNEL_SPLIT]
 
 
 def _codes(rows, k, gen, low=-128, pad=0):
