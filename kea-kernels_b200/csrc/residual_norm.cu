@@ -140,9 +140,11 @@ cudaError_t launch_direct(const kea::ResidualNormArgs &a, const kea_host::Device
         vpt /= 2;
     const int tpr = threads_for(a.D, vpt), threads = std::max(tpr, 128);
     const Launch l(ceil_div(a.M, threads / tpr), threads, 0, pdl, stream);
-#define KEA_RN(VPT, VEC) cudaLaunchKernelEx(&l.cfg, kea::residual_norm_kernel<TX, TY, VPT, VEC>, a, tpr)
-    if (vec) return vpt == 8 ? KEA_RN(8, true) : vpt == 16 ? KEA_RN(16, true) : KEA_RN(32, true);
-    return vpt == 8 ? KEA_RN(8, false) : vpt == 16 ? KEA_RN(16, false) : KEA_RN(32, false);
+#define KEA_RN(VPT, VEC, THREADS) cudaLaunchKernelEx(&l.cfg, kea::residual_norm_kernel<TX, TY, VPT, VEC, THREADS>, a, tpr)
+    if (vec)
+        return vpt == 8 ? KEA_RN(8, true, 512) : vpt == 16 ? (threads == 128 ? KEA_RN(16, true, 128) : KEA_RN(16, true, 512))
+                                               : (threads == 128 ? KEA_RN(32, true, 128) : KEA_RN(32, true, 512));
+    return vpt == 8 ? KEA_RN(8, false, 512) : vpt == 16 ? KEA_RN(16, false, 512) : KEA_RN(32, false, 512);
 #undef KEA_RN
 }
 

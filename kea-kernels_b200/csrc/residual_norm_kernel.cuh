@@ -88,6 +88,32 @@ KEA_DEVI void put(T *p, const float *v) {
 template <> KEA_DEVI uint32_t pack2<float>(float, float) { return 0u; }
 template <> KEA_DEVI float2 unpack2<float>(uint32_t) { return make_float2(0.f, 0.f); }
 
+// W values as they came from memory: 16-bit types stay packed until they are used (half the registers).
+template <typename T, int W>
+struct RawValues {
+    static constexpr bool kPacked = sizeof(T) == 2 && W == 8;
+    uint4 words;
+    float v[kPacked ? 1 : W];
+    KEA_DEVI void load(const T *p) {
+        if constexpr (kPacked) words = *reinterpret_cast<const uint4 *>(p);
+        else get<W>(p, v);
+    }
+    KEA_DEVI void values(float *f) const {
+        if constexpr (kPacked) {
+            const uint32_t u[4] = {words.x, words.y, words.z, words.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 t = unpack2<T>(u[i]);
+                f[2 * i] = t.x;
+                f[2 * i + 1] = t.y;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) f[i] = v[i];
+        }
+    }
+};
+
 // Sum or maximum over a row group's threads in a fixed order; `slot`: kRnMaxThreads / 32 floats used by this reduction
 // alone. Every thread of the CTA calls it.
 template <bool MAX>
@@ -167,19 +193,6 @@ struct RowPart {
             }
         }
     }
-    template <typename T>
-    KEA_DEVI void gate(float (&v)[VPT], const T *g, int act) const {
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            float gv[W];
-            get<W>(g + safe(c), gv);
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                if (act == KEA_GATE_SIGMOID) gv[i] = __fdividef(1.0f, 1.0f + __expf(-gv[i]));
-                v[W * c + i] *= gv[i];
-            }
-        }
-    }
     // h as INT8 codes with one scale, as the quantizer's single part
     KEA_DEVI void codes(const float (&v)[VPT], int8_t *q, int ldq, float *qs, bool live, float *slot) const {
         float amax = 0.f;
@@ -211,29 +224,60 @@ struct RowPart {
     }
 };
 
-template <typename TX, typename TY, int VPT, bool VEC>
-__global__ void __launch_bounds__(kRnMaxThreads) residual_norm_kernel(const ResidualNormArgs a, int tpr) {
+// THREADS: the largest CTA. With 128 (rows of up to 4096 values) four or, in 16-bit types, five CTAs share an SM.
+template <typename TX, typename TY, int VPT, bool VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS != 128 ? 1 : sizeof(TX) + sizeof(TY) == 4 ? 5 : 4) residual_norm_kernel(const ResidualNormArgs a, int tpr) {
     __shared__ float slots[kRnSlots * (kRnMaxThreads / 32)];
-    constexpr int S = kRnMaxThreads / 32, W = VEC ? 8 : 1;
+    constexpr int S = kRnMaxThreads / 32, W = VEC ? 8 : 1, C = VPT / W;
     const int rows = blockDim.x / tpr;
     const int row = blockIdx.x * rows + threadIdx.x / tpr;
     const bool live = row < a.M;
-    const long long m = live ? row : a.M - 1;   // a group past the last row does that one again and stores nothing
+    const int m = live ? row : a.M - 1;   // a group past the last row does that one again and stores nothing
     const RowPart<VPT, W> part{(int)(threadIdx.x % tpr), tpr, a.D};
     grid_dependency_wait();
     grid_launch_dependents();
+    // everything is asked for at once: the stream and the gate wait, as they came, for the block's norm. (Not an FP32 gate
+    // beside 32 FP32 values of each: the registers spill, 32000 rows of 1024 take 139 us instead of 98.)
+    constexpr bool kGateAhead = VPT < 32 || sizeof(TY) == 2;
+    RawValues<TX, W> xr[C];
+    RawValues<TY, W> gr[C];
     float u[VPT], x[VPT];
-    part.load(static_cast<const TY *>(a.y) + m * a.ldy, u);
-    part.load(static_cast<const TX *>(a.x) + m * a.ldx, x);
-    if (a.post) part.norm(u, a.post, a.post_w, a.post_b, a.post_eps, slots);
-    if (a.gate)
-        part.gate(u, static_cast<const TY *>(a.gate) + m / a.frames * a.gate_clip + m % a.frames * a.gate_row, a.gate_act);
-    // in place, the last row is still to be read by the groups that do it again
-    if (a.r == a.x && (blockIdx.x + 1) * rows > a.M) __syncthreads();
+    const TX *const xp = static_cast<const TX *>(a.x) + m * a.ldx;
+    const TY *const gp = static_cast<const TY *>(a.gate) + (long long)(m / a.frames) * a.gate_clip + (long long)(m % a.frames) * a.gate_row;
+    {
+        RawValues<TY, W> yr[C];
+        const TY *const yp = static_cast<const TY *>(a.y) + m * a.ldy;
 #pragma unroll
-    for (int c = 0; c < VPT / W; ++c)
+        for (int c = 0; c < C; ++c) yr[c].load(yp + part.safe(c));
+#pragma unroll
+        for (int c = 0; c < C; ++c) xr[c].load(xp + part.safe(c));
+        if (kGateAhead && a.gate)
+#pragma unroll
+            for (int c = 0; c < C; ++c) gr[c].load(gp + part.safe(c));
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            yr[c].values(u + W * c);
+#pragma unroll
+            for (int i = 0; i < W; ++i) u[W * c + i] = part.in(c) ? u[W * c + i] : 0.f;
+        }
+    }
+    if (a.post) part.norm(u, a.post, a.post_w, a.post_b, a.post_eps, slots);
+    if (a.gate) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float g[W];
+            if constexpr (kGateAhead) gr[c].values(g);
+            else get<W>(gp + part.safe(c), g);
+#pragma unroll
+            for (int i = 0; i < W; ++i) u[W * c + i] *= a.gate_act == KEA_GATE_SIGMOID ? __fdividef(1.0f, 1.0f + __expf(-g[i])) : g[i];
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        xr[c].values(x + W * c);
 #pragma unroll
         for (int i = 0; i < W; ++i) x[W * c + i] = part.in(c) ? fmaf(a.scale, u[W * c + i], x[W * c + i]) : 0.f;
+    }
     part.store(static_cast<TX *>(a.r) + m * a.ldr, x, live);
     if (a.pre) part.norm(x, a.pre, a.pre_w, a.pre_b, a.pre_eps, slots + 2 * S);
     if (a.h) {
