@@ -444,7 +444,7 @@ int8_gemm_tile_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             __syncwarp();
         }
     } else if constexpr (SPLIT) {   // one tile per cluster
-        const int ew = warp - 2, quad = warp & 3, mt = worker / p.n_tiles, m0 = mt * 128, n0 = (worker - mt * p.n_tiles) * BN;
+        const int ew = warp - 2, quad = warp & 3, n0 = worker % p.n_tiles * BN;
         const uint32_t consts = CONST0 + (uint32_t)(ew * Tile::CW) * 8u;
 #pragma unroll
         for (int i = 0; i < Tile::CW; i += 32) {
@@ -512,7 +512,7 @@ int8_gemm_tile_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     else __syncthreads();
     if constexpr (SPLIT) {
         if (warp >= 2) {   // every slice's sums have arrived
-            const int ew = warp - 2, quad = warp & 3, mt = worker / p.n_tiles, m0 = mt * 128, n0 = (worker - mt * p.n_tiles) * BN;
+            const int ew = warp - 2, quad = warp & 3, mt = worker / p.n_tiles, m0 = mt * 128, n0 = (worker - mt * p.n_tiles) * BN;   // the cluster's tile
             const int m = m0 + quad * 32 + lane;
             const float s = m < p.a.M ? p.a.qs[m] : 0.f;
             int8_finish_split<T, SILU>(p, STG0, CONST0 + (uint32_t)(ew * Tile::CW) * 8u, BN / p.splits, slice, quad, m0, n0, pair_of(s, s));

@@ -139,11 +139,12 @@ cudaError_t launch_direct(const kea::ResidualNormArgs &a, const kea_host::Device
     while (vpt > 8 && (!many || threads_for(a.D, vpt / 2) == threads_for(a.D, vpt)) && threads_for(a.D, vpt / 2) <= kea::kRnMaxThreads)
         vpt /= 2;
     const int tpr = threads_for(a.D, vpt), threads = std::max(tpr, 128);
+    if (vec && vpt == 32 && tpr * 24 >= a.D && threads == 128) vpt = 24;   // a quarter of the registers would be empty
     const Launch l(ceil_div(a.M, threads / tpr), threads, 0, pdl, stream);
 #define KEA_RN(VPT, VEC, THREADS) cudaLaunchKernelEx(&l.cfg, kea::residual_norm_kernel<TX, TY, VPT, VEC, THREADS>, a, tpr)
     if (vec)
         return vpt == 8 ? KEA_RN(8, true, 512) : vpt == 16 ? (threads == 128 ? KEA_RN(16, true, 128) : KEA_RN(16, true, 512))
-                                               : (threads == 128 ? KEA_RN(32, true, 128) : KEA_RN(32, true, 512));
+               : vpt == 24 ? KEA_RN(24, true, 128) : threads == 128 ? KEA_RN(32, true, 128) : KEA_RN(32, true, 512);
     return vpt == 8 ? KEA_RN(8, false, 512) : vpt == 16 ? KEA_RN(16, false, 512) : KEA_RN(32, false, 512);
 #undef KEA_RN
 }
