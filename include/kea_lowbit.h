@@ -1,5 +1,6 @@
 /*
- * kea_lowbit.h - C ABI of the B200 (sm_100a) low-bit GEMM library `libkea_lowbit.so`.
+ * kea_lowbit.h - C ABI of the B200 (sm_100a) low-bit GEMM library `libkea_lowbit.so`. At its end the operators around an
+ * 8-bit model: the linear map in 8-bit integers, the gated norm step between two blocks, and a beam search's step.
  *
  * The library multiplies INT8 activation parts by 1-bit (sign) or 2-bit (ternary) packed weights on the
  * tcgen05 tensor cores (kind::i8, INT32 accumulators in tensor memory) and applies the kea-kernels FP32
@@ -347,7 +348,11 @@ typedef struct KeaInt8Desc {
     uint32_t *error_word;     /* device word OR-ed with KEA_DEVERR_* bits, or NULL for the library's own */
 } KeaInt8Desc;
 
-enum { KEA_INT8_SILU = 1, KEA_INT8_PDL = 2 };
+enum {
+    KEA_INT8_SILU = 1,
+    KEA_INT8_PDL = 2              /* launch with programmatic dependent launch; the weights may be read before the previous
+                                     kernel of the stream has ended, so that kernel may not write them */
+};
 enum {
     KEA_INT8_KERNEL_REG = 1,      /* warp-level MMAs on operands loaded straight into registers: few tokens */
     KEA_INT8_KERNEL_TILE64 = 2,   /* tcgen05, tiles of 128 tokens x 64 channels */
@@ -388,7 +393,7 @@ typedef struct KeaResidualNormDesc {
 
 enum { KEA_NORM_NONE = 0, KEA_NORM_LAYER = 1, KEA_NORM_RMS = 2 };
 enum { KEA_GATE_NONE = 0, KEA_GATE_SIGMOID = 1 };
-enum { KEA_RNORM_PDL = 1 };
+enum { KEA_RNORM_PDL = 1 };       /* programmatic dependent launch; as above, for the norms' parameters */
 
 int kea_lowbit_residual_norm(const KeaResidualNormDesc *desc, void *stream);
 
@@ -415,7 +420,7 @@ typedef struct KeaBeamDesc {
     int32_t flags;                /* KEA_BEAM_* */
 } KeaBeamDesc;
 
-enum { KEA_BEAM_PDL = 1 };
+enum { KEA_BEAM_PDL = 1 };        /* programmatic dependent launch */
 
 int kea_lowbit_beam_select(const KeaBeamDesc *desc, void *stream);
 

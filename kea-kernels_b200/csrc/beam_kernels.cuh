@@ -13,7 +13,7 @@
 // The width-th largest of the lane maxima of all the CTA's warps at a hypothesis bounds its best logits from below: only
 // the few tiles whose maximum reaches it are read again (from the caches), and what reaches it in them, a little more
 // than `width` values in all, enters the warp's list. (Keeping the lists up to date while streaming made every warp pay
-// for its own `width` best: 3300 instructions for 2048 logits, 4096 x 8 x 131072 FP32 logits 43 us.) Candidates are
+// for its own `width` best: 3300 instructions for 2048 logits; one clip of 8 x 131072 FP32 logits 43 us, now 24.) Candidates are
 // gathered in shared memory and enter 32 at a time: every lane counts how many candidates and list entries are ahead of
 // its own, independent comparisons.
 // The units' sums and lists meet in the first CTA of the cluster (distributed shared memory), which forms every lse_k and

@@ -13,7 +13,13 @@
 // Work split. A CTA owns 16 channels (8 where that leaves SMs without one: the MMA's upper rows stay empty) x 8 RG tokens; its
 // 8 warps are slices of K, whose INT32 sums meet in shared memory, are added in slice order (exact) and finished. A warp
 // keeps D steps in flight, so with K <= 512 D its whole share is asked for at once.
-// Weights do not depend on the previous kernel of the stream: the first loads are issued before griddepcontrol.wait.
+// Weights do not depend on the previous kernel of the stream (KEA_INT8_PDL promises it): the first loads are issued before
+// griddepcontrol.wait.
+//
+// Measured on a B200 (launches back to back, without programmatic launch): 1 x 4096 x 1024 3.4 us (1.2 TB/s of weights; the
+// library's smallest kernels take 2.1 us), 8 x 1024 x 4096 3.7 us, 32 x 4096 x 1024 4.4 us. The first form of this kernel
+// (two steps in flight) took 6.5, 13.6 and 9.0 us. From some 64 tokens on every further 32 read all the weights again from L2
+// (128 x 4096 x 1024: 13.4 us), and the tcgen05 tiles, which share them, take over.
 #pragma once
 
 #include "int8_epilogue.cuh"

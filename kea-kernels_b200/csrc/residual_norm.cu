@@ -130,9 +130,9 @@ cudaError_t launch_flat(const FlatPlan &f, int device, bool pdl, void *stream) {
 template <typename TX, typename TY>
 cudaError_t launch_direct(const kea::ResidualNormArgs &a, const kea_host::Device &dev, bool vec, bool pdl, void *stream) {
     // One warp per row, up to 32 values per thread, as long as that gives every SM eight warps: no barriers, and the
-    // loads of 16 rows are in flight on an SM (32000 rows of 1024 FP32 values: 84 us, against 129 and 128 us with two and
+    // loads of 16 rows are in flight on an SM (32000 rows of 1024 FP32 values: 83 us, against 129 and 128 us with two and
     // four warps per row). Value by value at most 16 per thread: more is straight-line code that misses the instruction
-    // cache (8000 rows of 4095 values: 225 us, 464 with 32). Fewer rows: eight, the shortest chain of loads and sums.
+    // cache (8000 rows of 4095 values: 225-233 us, 464 with 32). Fewer rows: eight, the shortest chain of loads and sums.
     const int most = vec || threads_for(a.D, 16) > kea::kRnMaxThreads ? 32 : 16;
     const bool many = (long long)a.M * threads_for(a.D, most) >= 32LL * 8 * dev.sms;
     int vpt = most;

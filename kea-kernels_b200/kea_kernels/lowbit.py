@@ -4,10 +4,16 @@
   * quantize       - FP32 rows -> P residual INT8 parts + per-row part scales (optional LayerNorm / input SiLU);
   * gemm           - INT8 parts x packed weights -> exact INT32 accumulators -> the FP32 epilogue -> FP32 / FP16.
 
-They replace the reference's per-kernel NVRTC launches (src/kea_kernels/binary/layer.py:154-209,
+And the operators around an 8-bit model (C++ entry points, csrc/binding.cpp; the same checks, streams and errors):
+
+  * int8_linear    - INT8 codes x INT8 weights with a scale per token and per channel;
+  * residual_norm, residual_norm_quantized - the step between two blocks: norm after, gate, residual scale, norm before;
+  * beam_select, beam_reorder - a beam search's choice over hypotheses and labels, and its states' reordering.
+
+The first three replace the reference's per-kernel NVRTC launches (src/kea_kernels/binary/layer.py:154-209,
 src/kea_kernels/binary/layer_parts.py:112-130) and Triton launches (src/kea_kernels/ternary/fused_kernels.py:139-160).
-No call allocates on the launch path except where a function returns new tensors (quantize, prepare_panels); gemm
-writes caller-owned outputs, so it can be captured in a CUDA graph.
+No call allocates on the launch path except where a function returns new tensors; gemm writes caller-owned outputs, so it
+can be captured in a CUDA graph (the others too: their tensors then belong to the graph's pool).
 """
 from __future__ import annotations
 
