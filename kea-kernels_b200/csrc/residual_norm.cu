@@ -80,7 +80,7 @@ struct FlatPlan {
 
 // Whether the rows are contiguous in aligned buffers, enough to give every SM's warps one, and their parameters fit.
 bool plan_flat(const KeaResidualNormDesc *d, const kea::ResidualNormArgs &a, const kea_host::Device &dev, FlatPlan *f) {
-    const bool gate_shared = d->gate && d->gate_row_stride == 0 && d->gate_clip_stride == 0;
+    const bool gate_shared = d->gate && d->gate_row_stride == 0 && (d->gate_clip_stride == 0 || d->m <= d->frames);
     const auto contiguous = [&](const void *p, int64_t ld, int type) { return !p || (ld == d->d && aligned(p, 8 * type_size(type))); };
     if (!contiguous(d->x, d->ldx, d->x_type) || !contiguous(d->r, d->ldr, d->x_type) || !contiguous(d->y, d->ldy, d->y_type) ||
         !contiguous(d->h, d->ldh, d->h_type))
@@ -91,6 +91,9 @@ bool plan_flat(const KeaResidualNormDesc *d, const kea::ResidualNormArgs &a, con
     // narrower rows leave most of a warp's 128 groups empty (8000 rows of 100 values: 29 us against 14 us straight)
     if (d->d <= 512 || f->tpr > 128 || d->m < groups * dev.sms) return false;
     f->p.a = a;
+    f->p.gate_end = 0;
+    if (d->gate && d->gate_clip_stride >= 0 && d->gate_row_stride >= 0 && aligned(d->gate, 16))
+        f->p.gate_end = (d->m - 1) / d->frames * d->gate_clip_stride + (d->m - 1) % d->frames * d->gate_row_stride + d->d;
     f->p.padded = f->tpr * kea::kFlatVpt + 16;
     const bool held[5] = {d->post != KEA_NORM_NONE, d->post == KEA_NORM_LAYER && d->post_bias, d->pre != KEA_NORM_NONE,
                           d->pre == KEA_NORM_LAYER && d->pre_bias, gate_shared};

@@ -215,3 +215,22 @@ def test_refusals():
     r, h = call(x[:, :0], y[:, :0], pre_norm=pre)
     assert r.shape == h.shape == (2, 0, 64)
     assert _lib.read_device_error() == 0
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+@pytest.mark.parametrize("clips,frames,d,pad,offset", [(5, 501, 1001, 0, 0), (3, 1001, 519, 0, 0), (2, 1500, 2047, 3, 0), (5, 601, 1003, 5, 8),
+                                                       (4, 700, 997, 1, 3), (1, 2999, 1001, 0, 0), (9, 300, 517, 2, 16), (3, 900, 4089, 0, 0)])
+def test_gates_of_clips_beside_rows_of_odd_width(clips, frames, d, pad, offset, ty):
+    """A gate per clip inside a wider buffer that holds NaN beside it: each alignment against the rows, the buffer's end
+    right after the last value, and bases that leave no alignment."""
+    x, y, _, g = _inputs((clips, frames, d), F32, ty, seed=d + pad)
+    values = (0.5 + torch.randn(clips, d, generator=g)).to(DEV, ty)
+    flat = torch.full((offset + (clips - 1) * (d + pad) + d,), float("nan"), device=DEV, dtype=ty)
+    gate = flat[offset:].as_strided((clips, d), (d + pad, 1))
+    gate.copy_(values)
+    post, pre = _norm("rms", d, g), _norm("rms", d, g)
+    want_r, want_h = _exact(x, y, post, values, "none", 0.5, pre)
+    r, h = lowbit.residual_norm(x, y, post_norm=post, gate=gate, scale=0.5, pre_norm=pre)
+    _near(r, want_r)
+    _near(h, want_h, _enlarged(x, want_r, pre))
+    assert torch.equal(gate, values) and _lib.read_device_error() == 0
