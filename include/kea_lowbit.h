@@ -405,7 +405,7 @@ int kea_lowbit_residual_norm(const KeaResidualNormDesc *desc, void *stream);
  * not offered counts as -inf: where fewer than `width` are offered, the places left take such continuations by their flat
  * index, with score -inf.
  * logits: (b, k, v) at logits + b * ld_clip + k * ld_beam + v, any stride; scores FP32 [clips][beams]. beams and width <= 32,
- * width <= beams * vocab < 2^31. The outputs may not overlap the inputs. */
+ * width <= beams * vocab <= 2^31 - 4096. The outputs may not overlap the inputs. */
 typedef struct KeaBeamDesc {
     const void *logits;
     int64_t ld_clip, ld_beam;     /* elements */

@@ -13,6 +13,10 @@ using kea_host::ceil_div;
 
 size_t type_size(int type) { return type == KEA_TYPE_F32 ? 4 : 2; }
 
+// Indices of labels are 32 bits. A unit's end, a lane's next label and the label after the last vector are formed before they
+// are compared with the row's end: at most 512 (units of a row) + 32 and 31 past it.
+constexpr long long kMaxLabels = (1LL << 31) - 4096;
+
 int validate(const KeaBeamDesc *d) {
     if (!d || d->clips < 0 || d->beams < 1 || d->vocab < 1 || d->width < 1 || d->end < -1 || d->end >= d->vocab ||
         d->logits_type < KEA_TYPE_F32 || d->logits_type > KEA_TYPE_BF16 || (d->flags & ~KEA_BEAM_PDL))
@@ -20,7 +24,7 @@ int validate(const KeaBeamDesc *d) {
     if (d->clips == 0) return KEA_OK;
     if (!d->logits || !d->scores || !d->out_scores || !d->parents || !d->labels || (d->ended && d->end < 0))
         return KEA_ERR_INVALID_VALUE;
-    if (d->beams > kea::kBeamMax || d->width > kea::kBeamMax || (long long)d->beams * d->vocab >= (1LL << 31) ||
+    if (d->beams > kea::kBeamMax || d->width > kea::kBeamMax || (long long)d->beams * d->vocab > kMaxLabels ||
         d->width > (long long)d->beams * d->vocab || (long long)d->clips * kea::kBeamCluster >= (1LL << 31))
         return KEA_ERR_UNSUPPORTED;
     if (!aligned(d->logits, type_size(d->logits_type)) || !aligned(d->scores, 4) || !aligned(d->out_scores, 4) ||
