@@ -400,10 +400,11 @@ int kea_lowbit_residual_norm(const KeaResidualNormDesc *desc, void *stream);
 /* One step of a beam search: the `width` best continuations of every clip's hypotheses.
  *   c[b, k, v] = scores[b, k] + log_softmax(logits[b, k, :])[v]      (FP32), flat index k * vocab + v;
  * an ended hypothesis offers only the label `end`, at its own score. The continuations come in descending order, equal
- * ones by their flat index; within a hypothesis the logits themselves are compared. A logit that is -inf or not a number
- * is masked; a hypothesis whose score or log-sum is not finite (no label left, a logit of +inf) offers nothing. What is
- * not offered counts as -inf: where fewer than `width` are offered, the places left take such continuations by their flat
- * index, with score -inf.
+ * ones by their hypothesis; within a hypothesis the logits themselves are compared, equal logits by their label, so which
+ * labels are chosen does not depend on how many of them round to one score. A logit that is -inf or not a number is
+ * masked; a hypothesis whose score or log-sum is not finite (no label left, a logit of +inf) offers nothing. What is not
+ * offered counts as -inf, as does a score that FP32 does not hold: where fewer than `width` are left, the places take such
+ * continuations by their flat index, with score -inf. (A log-sum's last bits depend on how a row is split over warps.)
  * logits: (b, k, v) at logits + b * ld_clip + k * ld_beam + v, any stride; scores FP32 [clips][beams]. beams and width <= 32,
  * width <= beams * vocab <= 2^31 - 4096. The outputs may not overlap the inputs. */
 typedef struct KeaBeamDesc {

@@ -16,8 +16,10 @@
 // for its own `width` best: 3300 instructions for 2048 logits; one clip of 8 x 131072 FP32 logits 43 us, now 24.) Candidates are
 // gathered in shared memory and enter 32 at a time: every lane counts how many candidates and list entries are ahead of
 // its own, independent comparisons.
-// The units' sums and lists meet in the first CTA of the cluster (distributed shared memory), which forms every lse_k and
-// merges the lists by (c, flat index). No scratch memory, one launch.
+// The units' sums and lists meet in the first CTA of the cluster (distributed shared memory), which forms every lse_k, merges
+// each hypothesis' lists by (logit, label) and then the hypotheses' by (c, hypothesis, place). Many logits can have one c:
+// ordering the units' lists by c and label would choose by how a row was split, a unit's list being by logit. No scratch
+// memory, one launch.
 #pragma once
 
 #include "operator_common.cuh"
@@ -99,6 +101,25 @@ KEA_DEVI void beam_merge(BeamScratch &s, int n, int width, int lane, uint64_t &l
     __syncwarp();
     if (lane < width) list = s.list[lane];
     __syncwarp();
+}
+
+KEA_DEVI uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
+
+// A sequence that falls and rises (or the other way round) over each group of P lanes, P a power of two, in descending order.
+KEA_DEVI uint64_t beam_order(uint64_t v, int P, int lane) {
+    for (int j = P / 2; j > 0; j /= 2) {
+        const uint64_t u = __shfl_xor_sync(0xFFFFFFFFu, v, j);
+        v = ((lane & j) == 0) == (u > v) ? u : v;
+    }
+    return v;
+}
+
+// Merges `lists` sorted lists, list i in lanes i P .. i P + P - 1 of e, into the warp's (in the first P lanes): the larger of one
+// list's entry and the other's from its end are the best P of both.
+KEA_DEVI void beam_merge_lists(uint64_t e, int lists, int P, int lane, uint64_t &list) {
+    for (int w = P; w < P * lists; w *= 2) e = beam_order(larger(e, __shfl_xor_sync(0xFFFFFFFFu, e, w | (P - 1))), P, lane);
+    if (__any_sync(0xFFFFFFFFu, list != 0)) list = beam_order(larger(list, __shfl_xor_sync(0xFFFFFFFFu, e, P - 1)), P, lane);
+    else list = e;
 }
 
 struct BeamScan {
@@ -321,6 +342,7 @@ template <typename T, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS) beam_select_kernel(const BeamArgs a) {
     __shared__ double ul[kBeamSlots];                  // the units' log-sums
     __shared__ uint64_t ue[kBeamSlots * kBeamMax];     // and lists: [slot][width]
+    __shared__ uint64_t lists[kBeamMax * kBeamMax];    // (first CTA) the hypotheses' lists: [hypothesis][width]
     __shared__ float tops[2 * WARPS];                  // per warp: two of its largest lane maxima
     __shared__ float score[kBeamMax], lse[kBeamMax];   // per hypothesis; lse not a number: it offers nothing
     __shared__ bool over[kBeamMax];                    // it has ended
@@ -383,52 +405,72 @@ __global__ void __launch_bounds__(32 * WARPS) beam_select_kernel(const BeamArgs 
             const int r = a.rounds == 1 ? 0 : u / warps, w = u - r * warps;
             return map_to_rank(smem_u32(base) + 8u * (uint32_t)((r * WARPS + w % WARPS) * each + i), (uint32_t)(w / WARPS));
         };
-        for (int k = warp; k < K; k += WARPS) {
-            if (over[k]) continue;   // it needs none
-            double top = -INFINITY;
-            for (int g = lane; g < a.segs; g += 32) top = fmax(top, ld_cluster_f64(at(ul, k * a.segs + g, 1, 0)));
-            if (a.segs > 1)
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-            top = __shfl_sync(0xFFFFFFFFu, top, 0);
-            float s = 0.f;   // a segment with a logit of +inf is not a number, and makes the whole so
-            for (int g = lane; g < a.segs; g += 32) s += expf((float)(ld_cluster_f64(at(ul, k * a.segs + g, 1, 0)) - top));
-            if (a.segs > 1)
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-            if (lane == 0) {
-                // nothing is offered where it is infinite (no label left) or not a number
-                const float l = (float)(top + (double)logf(s));
-                lse[k] = fabsf(l) < INFINITY ? l : __int_as_float(0x7FC00000);
+        int P = 1;   // lists come in P places, `each` per turn; this lane's list and place in it
+        while (P < W) P *= 2;
+        const int each = 32 / P, mine = lane / P, q = lane - mine * P;
+        uint64_t list = 0;
+        // The hypotheses' log-sums, and their lists (by logit and label), shared by `parts` warps where they are few and long:
+        // as many as leave every warp one job.
+        const int parts = min(max(1, WARPS / K - 1), (a.segs + each - 1) / each);
+        for (int job = warp; job < K + K * parts; job += WARPS) {
+            if (job < K) {
+                const int k = job;
+                if (over[k]) continue;   // it needs none
+                double top = -INFINITY;
+                for (int g = lane; g < a.segs; g += 32) top = fmax(top, ld_cluster_f64(at(ul, k * a.segs + g, 1, 0)));
+                for (int o = 1; o < min(a.segs, 32); o *= 2) top = fmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+                top = __shfl_sync(0xFFFFFFFFu, top, 0);
+                float s = 0.f;   // a segment with a logit of +inf is not a number, and makes the whole so
+                for (int g = lane; g < a.segs; g += 32) s += expf((float)(ld_cluster_f64(at(ul, k * a.segs + g, 1, 0)) - top));
+                for (int o = 1; o < min(a.segs, 32); o *= 2) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+                if (lane == 0) {
+                    // nothing is offered where it is infinite (no label left) or not a number
+                    const float l = (float)(top + (double)logf(s));
+                    lse[k] = fabsf(l) < INFINITY ? l : __int_as_float(0x7FC00000);
+                }
+            } else {
+                const int k = (job - K) / parts, part = job - K - k * parts;
+                list = 0;
+                if (a.segs == 1) {
+                    if (lane < W) list = ld_cluster_u64(at(ue, k, W, lane));
+                } else {
+                    for (int g0 = part * each; g0 < a.segs; g0 += parts * each) {
+                        const int g = g0 + mine;
+                        beam_merge_lists(g < a.segs && q < W ? ld_cluster_u64(at(ue, k * a.segs + g, W, q)) : 0, min(each, a.segs - g0), P,
+                                         lane, list);
+                    }
+                }
+                if (lane < W) lists[(parts == 1 ? k : job) * W + lane] = list;
             }
         }
         __syncthreads();
-        // Merging in two levels: up to eight warps take the units' lists, whole lists to 32 lanes, then the first warp theirs.
-        uint64_t list = 0;
-        const auto enter = [&](uint64_t e) {   // 32 candidates: those that can enter, packed together
-            const bool good = e > __shfl_sync(0xFFFFFFFFu, list, W - 1);
-            const uint32_t pass = __ballot_sync(0xFFFFFFFFu, good);
-            if (pass == 0) return;
-            if (good) own.cand[__popc(pass & ((1u << lane) - 1u))] = e;
-            __syncwarp();
-            beam_merge(own, __popc(pass), W, lane, list);
-        };
-        const int each = 32 / W, mine = lane / W, q = lane - mine * W;   // lists per turn; this lane's list and place in it
-        const int takers = min(min(WARPS, 8), (a.units + each - 1) / each);
-        if (warp < takers)
-            for (int u0 = warp * each; u0 < a.units; u0 += takers * each) {
-                const int u = u0 + mine;
-                uint64_t e = 0;
-                if (mine < each && u < a.units) {
-                    const int k = a.segs == 1 ? u : u / a.segs;
-                    const float s = score[k], l = over[k] ? 0.f : lse[k];
-                    e = ld_cluster_u64(at(ue, u, W, q));
-                    if (e && l == l && fabsf(s) < INFINITY)
-                        e = beam_entry(over[k] ? s : __fadd_rn(__fsub_rn(entry_value(e), l), s), entry_index(e) + k * a.vocab);
-                    else
-                        e = 0;
+        if (parts > 1) {   // slots K .. K (1 + parts) - 1, below WARPS, hold the parts
+            if (warp < K) {
+                const int first = K + warp * parts;
+                list = lane < W ? lists[first * W + lane] : 0;
+                for (int p = 1; p < parts; p += each) {
+                    const int from = p + mine;
+                    beam_merge_lists(from < parts && q < W ? lists[(first + from) * W + q] : 0, min(each, parts - p), P, lane, list);
                 }
-                enter(e);
+                if (lane < W) lists[warp * W + lane] = list;
+            }
+            __syncthreads();
+        }
+        // The hypotheses' lists by c, hypothesis and place in the list: c does not rise along a list, so each stays in its order.
+        // Where one warp would take more than two turns, up to eight do and the first takes theirs.
+        const int turns = (K + each - 1) / each, takers = turns <= 2 ? 1 : min(min(WARPS, 8), turns);
+        list = 0;
+        if (warp < takers)
+            for (int k0 = warp * each; k0 < K; k0 += takers * each) {
+                const int k = k0 + mine;
+                uint64_t e = 0;
+                if (k < K && q < W) {
+                    const float s = score[k], l = over[k] ? 0.f : lse[k];
+                    e = lists[k * W + q];
+                    const float c = over[k] ? s : __fadd_rn(__fsub_rn(entry_value(e), l), s);
+                    e = e && l == l && fabsf(s) < INFINITY && c > -INFINITY ? beam_entry(c, k * kBeamMax + q) : 0;
+                }
+                beam_merge_lists(e, min(each, K - k0), P, lane, list);
             }
         if (takers > 1) {
             __syncwarp();
@@ -437,7 +479,7 @@ __global__ void __launch_bounds__(32 * WARPS) beam_select_kernel(const BeamArgs 
             if (warp == 0)
                 for (int w = 1; w < takers; w += each) {
                     const int from = w + mine;
-                    enter(mine < each && from < takers ? scratch[from].list[q] : 0);
+                    beam_merge_lists(from < takers && q < W ? scratch[from].list[q] : 0, min(each, takers - w), P, lane, list);
                 }
         }
         if (warp == 0) {
@@ -445,7 +487,11 @@ __global__ void __launch_bounds__(32 * WARPS) beam_select_kernel(const BeamArgs 
             // (at most 31 are taken, so 63 numbers are enough).
             const uint32_t some = __ballot_sync(0xFFFFFFFFu, lane < W && list != 0);
             float v = entry_value(list);
-            int i = entry_index(list);
+            int i = 0;   // the flat index
+            if (some >> lane & 1) {
+                const int place = entry_index(list), k = place / kBeamMax;
+                i = k * a.vocab + entry_index(lists[k * W + place % kBeamMax]);
+            }
             if (__popc(some) < W) {
                 uint32_t low = 0, high = 0;   // flat indices 0 .. 31 and 32 .. 63 that the list holds
                 if (some >> lane & 1) {

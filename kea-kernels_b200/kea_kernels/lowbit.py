@@ -403,9 +403,10 @@ def beam_select(logits: Tensor, scores: Tensor, width: int | None = None, *, end
     many as there are hypotheses by default) of every clip. logits [clips, beams, vocab] FP32, FP16 or BF16 with unit
     stride along the labels; scores FP32 [clips, beams], -inf for an absent hypothesis. `end` is the label that ends a
     hypothesis; an ended one (ended bool [clips, beams]) only offers `end` again, at its own score. Equal continuations
-    come by (hypothesis, label). Logits of -inf and those that are not numbers are masked; a hypothesis with an infinite
-    score or log-sum offers nothing; places that nothing fills take what is not offered by (hypothesis, label), with score
-    -inf. At most 32 hypotheses and places. `out`: tensors to write to (rows of a history, for instance)."""
+    come by hypothesis; one hypothesis' continuations come by logit, equal logits by label. Logits of -inf and those that
+    are not numbers are masked; a hypothesis with an infinite score or log-sum offers nothing; places that nothing fills
+    take what is not offered by (hypothesis, label), with score -inf. At most 32 hypotheses and places. `out`: tensors to
+    write to (rows of a history, for instance), which may not overlap the inputs."""
     step = (_lib._native or _lib.native()).beam_select(logits, scores, width, end, ended, out, pdl)
     return BeamStep._make(step) if out is None else out
 

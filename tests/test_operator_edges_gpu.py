@@ -27,3 +27,64 @@ def test_codes_past_32_bit_offsets():
     assert torch.equal(q[-some:], want_q) and torch.equal(qs[-some:], want_qs) and torch.equal(r[:, -some:], want_r)
     assert bool((qs[:-some] == 1e-30).all()) and not bool(q[:3].any()) and not bool(q[-some - 3:-some].any())
     assert _lib.read_device_error() == 0
+
+
+def _ulps(base, count, gen):
+    """`count` neighbouring FP32 numbers from base up, in a random order."""
+    bits = torch.tensor([base], dtype=torch.float32).view(torch.int32) + torch.randperm(count, generator=gen).int()
+    return bits.view(torch.float32)
+
+
+@pytest.mark.parametrize("clips", [1, 2, 40, 300])
+@pytest.mark.parametrize("vocab", [40, 1025, 30000])
+def test_a_hypothesis_labels_come_by_logit(vocab, clips):
+    """Logits a rounding apart at scores where dozens of them have one score: a hypothesis' labels come by logit, equal
+    logits by label, whatever number of clips (and with it the split of a row) and whatever the width; a narrower choice is
+    the beginning of a wider one."""
+    gen = torch.Generator().manual_seed(vocab)
+    one = torch.randn(3, vocab, generator=gen).clamp(-3, 3)
+    for k in range(3):
+        at = torch.randperm(vocab, generator=gen)[:38]
+        one[k, at] = _ulps(5.0, 19, gen).repeat(2)                      # every logit twice
+    x = one.to(DEV).expand(clips, 3, vocab).contiguous()
+    # the other hypotheses' best are 100 and more below the first one's: all 32 places are its own
+    s = torch.tensor([-300.0, -400.0, -500.0], device=DEV).expand(clips, 3).contiguous()
+    order = torch.sort(one[0], descending=True, stable=True)[1]
+    wide = lowbit.beam_select(x, s, 32)
+    assert torch.equal(wide.tokens.cpu().long(), order[:32].expand(clips, 32)) and not bool(wide.parents.any())
+    assert len(wide.scores[0].unique()) < 8                             # they do tie
+    for width in (1, 2, 5, 31):
+        step = lowbit.beam_select(x, s, width)
+        assert torch.equal(step.tokens, wide.tokens[:, :width]) and torch.equal(step.parents, wide.parents[:, :width])
+
+
+@pytest.mark.parametrize("clips", [1, 40, 300])
+@pytest.mark.parametrize("vocab", [64, 1024, 30000])
+def test_hypotheses_that_tie_come_by_index(vocab, clips):
+    """Three hypotheses with the same logits and scores: of equal scores the lower hypothesis' come first, within it the
+    larger logit, then the lower label."""
+    gen = torch.Generator().manual_seed(vocab + 1)
+    one = torch.randn(vocab, generator=gen).clamp(-3, 3)
+    at = torch.randperm(vocab, generator=gen)[:38]
+    one[at] = _ulps(5.0, 38, gen)
+    x = one.to(DEV).expand(clips, 3, vocab).contiguous()
+    step = lowbit.beam_select(x, torch.full((clips, 3), -300.0, device=DEV), 32)
+    scores, parents, tokens = step.scores.tolist(), step.parents.tolist(), step.tokens.tolist()
+    order = torch.sort(one, descending=True, stable=True)[1].tolist()
+    for b in range(clips):
+        places = [(-scores[b][j], parents[b][j], -float(one[tokens[b][j]]), tokens[b][j]) for j in range(32)]
+        assert places == sorted(places)
+        for k in range(3):
+            mine = [tokens[b][j] for j in range(32) if parents[b][j] == k]
+            assert mine == order[:len(mine)]
+        assert 0 in parents[b] and len(set(scores[b])) < 8
+
+
+def test_a_score_below_the_range_is_not_offered():
+    """A score that FP32 does not hold is -inf, as what is masked: the places go by label."""
+    x = torch.zeros(1, 1, 6, device=DEV)
+    x[0, 0, 0], x[0, 0, 3], x[0, 0, 4], x[0, 0, 5] = -float("inf"), 2.9e38, -3e38, 3e38
+    step = lowbit.beam_select(x, torch.zeros(1, 1, device=DEV), 5)             # label 4: -3e38 - 3e38
+    assert step.tokens[0].tolist() == [5, 3, 1, 2, 0] and step.scores[0].isfinite().tolist() == [True] * 4 + [False]
+    step = lowbit.beam_select(x, torch.full((1, 1), -1e38, device=DEV), 5)     # labels 1 and 2: -3e38 - 1e38
+    assert step.tokens[0].tolist() == [5, 3, 0, 1, 2] and step.scores[0].isfinite().tolist() == [True] * 2 + [False] * 3
