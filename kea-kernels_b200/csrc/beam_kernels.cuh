@@ -274,27 +274,33 @@ struct BeamUnit {
         const float side[1] = {c.side};
         beam_add(c, side);
     }
-    // the values that reach `low`, into the list
+    // the values that reach `low`, into the list; tiles come by index, so once the list is full a later value has to exceed
+    // its last (a row of one value, or a segment that is masked whole, would be offered value by value)
     KEA_DEVI void gather(BeamScan &c, float low, int width, BeamScratch &s) const {
         BeamGather g(s, c.list, width, lane);
-        uint32_t todo = __ballot_sync(0xFFFFFFFFu, c.tiles >= float_key(low) && c.tiles > float_key(-INFINITY));
+        uint32_t need = max(float_key(low), float_key(-INFINITY) + 1);   // key of the least value that can enter
+        uint32_t todo = __ballot_sync(0xFFFFFFFFu, c.tiles >= need);
         while (todo) {
-            const int v1 = __ffs(todo) * group * TILE;
+            const int owner = __ffs(todo) - 1, v1 = (owner + 1) * group * TILE;
             todo &= todo - 1;
+            if (__shfl_sync(0xFFFFFFFFu, c.tiles, owner) < need) continue;
             for (int v0 = v1 - group * TILE; v0 < min(v1, vecs); v0 += TILE) {
                 uint4 w[V];
                 load(v0, w);
                 float x[E];
                 values(w, x);
+                const float least = key_float(need);
                 uint32_t mask = 0;   // this lane's values that do
 #pragma unroll
-                for (int e = 0; e < E; ++e) mask |= (x[e] >= low && x[e] > -INFINITY ? 1u : 0u) << e;
+                for (int e = 0; e < E; ++e) mask |= (x[e] >= least ? 1u : 0u) << e;
                 while (__any_sync(0xFFFFFFFFu, mask != 0)) {   // one of every lane at a time, hardly ever more than one
                     const int e = mask ? __ffs(mask) - 1 : 0;
                     const int i = first + (v0 + 32 * (e / N) + lane) * N + e % N;
                     g.offer(mask != 0, mask ? beam_entry(to_float(row[i]), i) : 0);
                     mask &= mask - 1;
                 }
+                const uint64_t end = __shfl_sync(0xFFFFFFFFu, c.list, width - 1);
+                if (end) need = max(need, (uint32_t)(end >> 32) + 1);
             }
         }
         g.offer(c.side >= low && c.side > -INFINITY, beam_entry(c.side, edge));

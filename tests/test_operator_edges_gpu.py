@@ -88,3 +88,32 @@ def test_a_score_below_the_range_is_not_offered():
     assert step.tokens[0].tolist() == [5, 3, 1, 2, 0] and step.scores[0].isfinite().tolist() == [True] * 4 + [False]
     step = lowbit.beam_select(x, torch.full((1, 1), -1e38, device=DEV), 5)     # labels 1 and 2: -3e38 - 1e38
     assert step.tokens[0].tolist() == [5, 3, 0, 1, 2] and step.scores[0].isfinite().tolist() == [True] * 2 + [False] * 3
+
+
+def _selection_us(x, s, width):
+    """The least of five times of one selection, launches back to back."""
+    for _ in range(3):
+        lowbit.beam_select(x, s, width)
+    least = float("inf")
+    for _ in range(5):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        for _ in range(20):
+            lowbit.beam_select(x, s, width)
+        b.record()
+        b.synchronize()
+        least = min(least, 50.0 * a.elapsed_time(b))
+    return least
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_one_value_take_no_longer(dtype):
+    """Every logit of such a row reaches the bound of its best. Offered one by one they take several times a usual row's
+    time; time between runs moves by a tenth, so 1.6 tells the two apart."""
+    x = torch.randn(8, 8, 262144, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(dtype)
+    s = -10.0 * torch.rand(8, 8, device=DEV)
+    usual = _selection_us(x, s, 8)
+    x[:] = 1.5
+    assert _selection_us(x, s, 8) < 1.6 * usual
+    x[..., ::2] = 1.0
+    assert _selection_us(x, s, 8) < 1.6 * usual
