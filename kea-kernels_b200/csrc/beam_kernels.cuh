@@ -5,10 +5,11 @@
 // its `width` largest logits are all it can contribute, and they can be found while the exponentials are summed, before
 // lse_k is known. One thread-block cluster serves a clip; each of its warps takes a unit (a hypothesis, or a segment of
 // one) and streams its logits once, a tile ahead, keeping
-//   * per lane a running maximum m and the sum of 2^(x log2 e - off), off = m log2 e rounded, in FP32; the log-sum is
-//     (off + log2 of the sum) / log2 e, so the rounding of off cancels. Where that is not finite - a logit that is not a
-//     number, or one so large that off overflows - the unit is summed again with its maximum known, masking what is not
-//     a number;
+//   * per lane a running maximum m and the sum of 2^((x - m) log2 e), in FP32: x - m is at most zero and loses nothing where
+//     it counts, at any level of the logits (masks of the type's lowest value, log-probabilities). With m log2 e rounded
+//     instead, one FMA less per value, its rounding passes the exponential's range below about -2^30. Where the sum is not
+//     a number - a logit that is not one beside others in a lane's tile, or +inf - the unit is summed again with its maximum
+//     known, masking what is not a number;
 //   * the maximum of every tile.
 // The width-th largest of the lane maxima of all the CTA's warps at a hypothesis bounds its best logits from below: only
 // the few tiles whose maximum reaches it are read again (from the caches), and what reaches it in them, a little more
@@ -123,8 +124,8 @@ KEA_DEVI void beam_merge_lists(uint64_t e, int lists, int P, int lane, uint64_t 
 }
 
 struct BeamScan {
-    float m = -INFINITY, off = 0.f;   // this lane's maximum and m log2 e (0 while there is none)
-    float s = 0.f;                    // sum of 2^(x log2 e - off)
+    float m = -INFINITY, from = 0.f;  // this lane's maximum; the same, 0 while there is none
+    float s = 0.f;                    // sum of 2^((x - from) log2 e)
     uint32_t tiles = 0;               // key of the largest logit in this lane's group of tiles
     float side = -INFINITY;           // this lane's value before the first or after the last vector
     uint64_t list = 0;                // lane i: the i-th best logit
@@ -145,20 +146,18 @@ KEA_DEVI float beam_add(BeamScan &c, const float (&x)[E]) {
 #pragma unroll
     for (int e = 0; e < E; ++e) tm = fmaxf(tm, x[e]);
     if (tm > c.m) {
-        const float off = tm * kLog2e;
-        c.s *= exp2_approx(c.off - off);   // 0 before the first finite logit
-        c.m = tm;
-        c.off = off;
+        c.s = c.m == -INFINITY ? 0.f : c.s * exp2_approx((c.m - tm) * kLog2e);   // nothing counts before the first finite logit
+        c.m = c.from = tm;
     }
     if constexpr (E == 1) {
-        c.s += exp2_approx(fmaf(x[0], kLog2e, -c.off));
+        c.s += exp2_approx((x[0] - c.from) * kLog2e);
     } else {
-        const uint64_t scale = pair_of(kLog2e, kLog2e), off = pair_of(-c.off, -c.off);
+        const uint64_t scale = pair_of(kLog2e, kLog2e), from = pair_of(-c.from, -c.from);
         uint64_t sum = pair_of(0.f, 0.f);
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
             float a, b;
-            unpair(fma2(pair_of(x[e], x[e + 1]), scale, off), a, b);
+            unpair(mul2(add2(pair_of(x[e], x[e + 1]), from), scale), a, b);
             sum = add2(sum, pair_of(exp2_approx(a), exp2_approx(b)));
         }
         float a, b;
@@ -311,18 +310,14 @@ struct BeamUnit {
 // log sum exp of logits lo .. hi - 1, the warp's lanes having scanned them; not a number: a logit of +inf.
 template <typename T>
 KEA_DEVI double beam_log_sum(const BeamScan &c, const T *row, int lo, int hi, int lane) {
-    constexpr double kLn2 = 0.6931471805599453;
     float m = c.m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     if (m == -INFINITY) return -INFINITY;
-    float off = c.m == -INFINITY ? -INFINITY : c.off;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) off = fmaxf(off, __shfl_xor_sync(0xFFFFFFFFu, off, o));
-    float s = c.m == -INFINITY ? c.s : c.s * exp2_approx(c.off - off);   // a lane of NaN alone keeps its NaN
+    float s = c.m == -INFINITY ? 0.f : c.s * exp2_approx((c.m - m) * kLog2e);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    if (s < INFINITY && fabsf(off) < INFINITY) return (double)off * kLn2 + (double)logf(s);
+    if (s < INFINITY) return (double)m + (double)logf(s);
     s = 0.f;
     for (int i = lo + lane; i < hi; i += 32) {
         const float x = to_float(row[i]);
@@ -344,8 +339,10 @@ KEA_DEVI uint64_t ld_cluster_u64(uint32_t addr) {
     return v;
 }
 
+// CTAs of 8 warps: four share an SM (with the 80 registers that the compiler would take for FP32, three: 256 x 8 x 1025 is then a
+// second wave, 16.5 instead of 12.2 us).
 template <typename T, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS) beam_select_kernel(const BeamArgs a) {
+__global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) beam_select_kernel(const BeamArgs a) {
     __shared__ double ul[kBeamSlots];                  // the units' log-sums
     __shared__ uint64_t ue[kBeamSlots * kBeamMax];     // and lists: [slot][width]
     __shared__ uint64_t lists[kBeamMax * kBeamMax];    // (first CTA) the hypotheses' lists: [hypothesis][width]
@@ -422,12 +419,14 @@ __global__ void __launch_bounds__(32 * WARPS) beam_select_kernel(const BeamArgs 
             if (job < K) {
                 const int k = job;
                 if (over[k]) continue;   // it needs none
-                double top = -INFINITY;
-                for (int g = lane; g < a.segs; g += 32) top = fmax(top, ld_cluster_f64(at(ul, k * a.segs + g, 1, 0)));
+                const double own_sum = lane < a.segs ? ld_cluster_f64(at(ul, k * a.segs + lane, 1, 0)) : (double)-INFINITY;
+                double top = fmax((double)-INFINITY, own_sum);   // (a number)
+                for (int g = lane + 32; g < a.segs; g += 32) top = fmax(top, ld_cluster_f64(at(ul, k * a.segs + g, 1, 0)));
                 for (int o = 1; o < min(a.segs, 32); o *= 2) top = fmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
                 top = __shfl_sync(0xFFFFFFFFu, top, 0);
-                float s = 0.f;   // a segment with a logit of +inf is not a number, and makes the whole so
-                for (int g = lane; g < a.segs; g += 32) s += expf((float)(ld_cluster_f64(at(ul, k * a.segs + g, 1, 0)) - top));
+                // a segment with a logit of +inf is not a number, and makes the whole so
+                float s = lane < a.segs ? expf((float)(own_sum - top)) : 0.f;
+                for (int g = lane + 32; g < a.segs; g += 32) s += expf((float)(ld_cluster_f64(at(ul, k * a.segs + g, 1, 0)) - top));
                 for (int o = 1; o < min(a.segs, 32); o *= 2) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
                 if (lane == 0) {
                     // nothing is offered where it is infinite (no label left) or not a number

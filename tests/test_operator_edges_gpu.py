@@ -117,3 +117,36 @@ def test_rows_of_one_value_take_no_longer(dtype):
     assert _selection_us(x, s, 8) < 1.6 * usual
     x[..., ::2] = 1.0
     assert _selection_us(x, s, 8) < 1.6 * usual
+
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_finite_masks_and_log_probabilities_take_one_pass(dtype):
+    """Logits far below zero, as a mask or everywhere, are summed in the pass that reads them. A second, scalar pass over the
+    masked rows is several times as long as the first; time between runs moves by a tenth, so 1.6 tells the two apart."""
+    vocab = 262144
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    plain = torch.randn(8, 8, vocab, generator=gen, device=DEV)
+    s = -10.0 * torch.rand(8, 8, generator=gen, device=DEV)
+    usual = _selection_us(plain.to(dtype), s, 8)
+    low = torch.finfo(dtype).min
+    for mask in (-1e4, max(-1e9, low), low):
+        x = plain.clone().to(dtype)
+        x[..., :vocab // 2] = mask
+        assert _selection_us(x, s, 8) < 1.6 * usual, mask
+    assert _selection_us((plain - 110.0).to(dtype), s, 8) < 1.6 * usual
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("level", [0.0, -90.0, -1e4, -1e9, -2.0 ** 27, -1e12, -1e30, -3.3e38])
+def test_log_sums_far_below_zero(level, dtype):
+    """Rows around any level, some with the lowest value beside: the score is the rounded logit less the log-sum. The
+    sum is good to 1e-6; then FP32 numbers of the level's size are subtracted: two roundings of it."""
+    gen = torch.Generator().manual_seed(3)
+    x = (level + 3.0 * torch.randn(4, 3, 700, generator=gen)).to(dtype)
+    x[1, :, 100:600] = torch.finfo(dtype).min
+    x[2, :, ::2] = -float("inf")
+    x[3, 1, 5:] = torch.finfo(dtype).min
+    step = lowbit.beam_select(x.to(DEV), torch.zeros(4, 3, device=DEV), 1)
+    want = torch.log_softmax(x.double(), -1).flatten(1).amax(-1)
+    assert bool(((step.scores.cpu()[:, 0].double() - want).abs() <= 2e-5 + 2.0 ** -22 * abs(level)).all())
