@@ -95,8 +95,8 @@ bool plan_flat(const KeaResidualNormDesc *d, const kea::ResidualNormArgs &a, con
     if (d->gate && d->gate_clip_stride >= 0 && d->gate_row_stride >= 0 && aligned(d->gate, 16))
         f->p.gate_end = (d->m - 1) / d->frames * d->gate_clip_stride + (d->m - 1) % d->frames * d->gate_row_stride + d->d;
     f->p.padded = f->tpr * kea::kFlatVpt + 16;
-    const bool held[5] = {d->post != KEA_NORM_NONE, d->post == KEA_NORM_LAYER && d->post_bias, d->pre != KEA_NORM_NONE,
-                          d->pre == KEA_NORM_LAYER && d->pre_bias, gate_shared};
+    const bool held[5] = {d->post != KEA_NORM_NONE, d->post != KEA_NORM_NONE && d->post_bias, d->pre != KEA_NORM_NONE,
+                          d->pre != KEA_NORM_NONE && d->pre_bias, gate_shared};
     int n = 0;
     f->p.params = 0;
     for (int k = 0; k < 5; ++k)

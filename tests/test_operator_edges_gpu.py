@@ -4,10 +4,13 @@ that are not what their class says, buffers that overlap, rows that are not numb
 Tolerances stand at each test; where none is named the values have to be equal."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
 from kea_kernels import _lib, lowbit
+from test_operators_cpu import ResidualNormDesc
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -150,3 +153,23 @@ def test_log_sums_far_below_zero(level, dtype):
     step = lowbit.beam_select(x.to(DEV), torch.zeros(4, 3, device=DEV), 1)
     want = torch.log_softmax(x.double(), -1).flatten(1).amax(-1)
     assert bool(((step.scores.cpu()[:, 0].double() - want).abs() <= 2e-5 + 2.0 ** -22 * abs(level)).all())
+
+
+@pytest.mark.parametrize("rows,d", [(3, 1001), (12024, 1001), (12024, 1000), (5, 64)])
+def test_a_bias_beside_root_mean_square_norms(rows, d):
+    """The C entry point takes a bias with either norm, on every route: many rows of odd width as few of them. A normed value
+    is off by 3e-6 of the row's largest (sums of at most 32 values per thread and 14 levels), twice, and r's error is
+    enlarged by at most 1 / 0.3 in the second norm: 3e-5 of the largest magnitude."""
+    gen = torch.Generator(device=DEV).manual_seed(d)
+    x, y = (torch.randn(rows, d, generator=gen, device=DEV) for _ in range(2))
+    w1, b1, w2, b2 = (torch.randn(d, generator=gen, device=DEV) + (i % 2 == 0) for i in range(4))
+    r, h = torch.empty_like(x), torch.empty_like(x)
+    desc = ResidualNormDesc(x=x.data_ptr(), y=y.data_ptr(), ldx=d, ldy=d, frames=rows, post=2, pre=2, scale=0.5, post_eps=1e-6,
+                            pre_eps=1e-6, post_weight=w1.data_ptr(), post_bias=b1.data_ptr(), pre_weight=w2.data_ptr(),
+                            pre_bias=b2.data_ptr(), r=r.data_ptr(), h=h.data_ptr(), ldr=d, ldh=d, m=rows, d=d)
+    _lib.check(_lib.lib().kea_lowbit_residual_norm(ctypes.byref(desc), _lib.stream_handle(x.device)), "residual_norm")
+    norm = lambda v, w, b: v / ((v * v).mean(-1, keepdim=True) + 1e-6).sqrt() * w.double() + b.double()  # noqa: E731
+    want_r = x.double() + 0.5 * norm(y.double(), w1, b1)
+    want_h = norm(want_r, w2, b2)
+    for got, want in ((r, want_r), (h, want_h)):
+        assert bool(((got.double() - want).abs() <= 3e-5 * want.abs().amax(-1, keepdim=True).clamp_min(1.0)).all())
