@@ -30,7 +30,7 @@ struct ResidualNormArgs {
     long long ldr, ldh;
     int h_type;
     int8_t *q;
-    long long ldq;                       // as every row stride: rows times it passes 32 bits
+    int ldq;                             // rows times it pass 32 bits: multiplied in 64
     float *qs;
     int M, D;
 };
@@ -194,7 +194,7 @@ struct RowPart {
         }
     }
     // h as INT8 codes with one scale, as the quantizer's single part
-    KEA_DEVI void codes(const float (&v)[VPT], int8_t *q, long long ldq, float *qs, bool live, float *slot) const {
+    KEA_DEVI void codes(const float (&v)[VPT], int8_t *q, int ldq, float *qs, bool live, float *slot) const {
         float amax = 0.f;
 #pragma unroll
         for (int c = 0; c < C; ++c)
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 4 : 1) residual_norm
         else if (a.h_type == KEA_TYPE_F16) part.store(static_cast<__half *>(a.h) + m * a.ldh, x, live);
         else part.store(static_cast<__nv_bfloat16 *>(a.h) + m * a.ldh, x, live);
     }
-    if (a.q) part.codes(x, a.q + m * a.ldq, a.ldq, a.qs + m, live, slots + 4 * S);
+    if (a.q) part.codes(x, a.q + (long long)m * a.ldq, a.ldq, a.qs + m, live, slots + 4 * S);
 }
 
 // ---- many contiguous rows of any width -----------------------------------------------------------------------------------
@@ -516,7 +516,7 @@ __global__ void __launch_bounds__(kFlatThreads, 1) residual_norm_flat_kernel(con
             for (int i = 0; i < kFlatVpt; ++i) amax = fmaxf(amax, fabsf(x[i]));
             amax = row_reduce<true>(amax, TPR, slots + 4 * SL);
             const float s = fmaxf(__fdiv_rn(amax, 127.0f), 1.0e-30f), inv = __frcp_rn(s);
-            int8_t *const q = a.q + m * a.ldq;
+            int8_t *const q = a.q + (long long)m * a.ldq;
 #pragma unroll
             for (int c = 0; c < kFlatGroups; ++c) {
                 float t[4];
