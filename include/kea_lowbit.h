@@ -371,7 +371,8 @@ int kea_lowbit_int8_gemm(const KeaInt8Desc *desc, void *stream);
  * root-mean-square norm v / sqrt(mean(v^2) + eps). gate (y_type, or NULL): value (row m, column i) at
  * gate + (m / frames) * gate_clip_stride + (m % frames) * gate_row_stride + i, so 0 strides share it; act: as is, or the
  * logistic function. q / qs: INT8 codes and one scale per row of h, as kea_lowbit_quantize forms one part (columns d ..
- * ldq - 1 written as 0). All arithmetic is FP32. d <= 16384. h and q may not overlap x, y or the gate. */
+ * ldq - 1 written as 0), but for a row of h that holds a NaN: its scale is NaN, its codes 0. All arithmetic is FP32.
+ * d <= 16384. h and q may not overlap x, y or the gate. */
 typedef struct KeaResidualNormDesc {
     const void *x, *y, *gate;
     int64_t ldx, ldy;             /* row strides in elements */

@@ -114,14 +114,28 @@ struct RawValues {
     }
 };
 
-// Sum or maximum over a row group's threads in a fixed order; `slot`: kRnMaxThreads / 32 floats used by this reduction
+// The larger of two values; not a number where one of them is none.
+KEA_DEVI float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// The largest size of three values, the same way.
+KEA_DEVI float max_size_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// Sum or maximum (max_nan) over a row group's threads in a fixed order; `slot`: kRnMaxThreads / 32 floats used by this reduction
 // alone. Every thread of the CTA calls it.
 template <bool MAX>
 KEA_DEVI float row_reduce(float v, int tpr, float *slot) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const float u = __shfl_xor_sync(0xFFFFFFFFu, v, o);
-        v = MAX ? fmaxf(v, u) : v + u;
+        v = MAX ? max_nan(v, u) : v + u;
     }
     if (tpr == 32) return v;
     const int warp = threadIdx.x >> 5, per = tpr >> 5;
@@ -129,7 +143,7 @@ KEA_DEVI float row_reduce(float v, int tpr, float *slot) {
     __syncthreads();
     const int first = warp - warp % per;
     float r = slot[first];
-    for (int w = 1; w < per; ++w) r = MAX ? fmaxf(r, slot[first + w]) : r + slot[first + w];
+    for (int w = 1; w < per; ++w) r = MAX ? max_nan(r, slot[first + w]) : r + slot[first + w];
     return r;
 }
 
@@ -193,15 +207,14 @@ struct RowPart {
             }
         }
     }
-    // h as INT8 codes with one scale, as the quantizer's single part
+    // h as INT8 codes with one scale, as the quantizer's single part; codes hold no NaN, so a row with one has scale NaN (and
+    // codes 0), and the product after it is not a number either
     KEA_DEVI void codes(const float (&v)[VPT], int8_t *q, int ldq, float *qs, bool live, float *slot) const {
         float amax = 0.f;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int i = 0; i < W; ++i) amax = fmaxf(amax, in(c) ? fabsf(v[W * c + i]) : 0.f);
+        for (int i = 0; i < VPT; i += 2) amax = max_size_nan(amax, in(i / W) ? v[i] : 0.f, in((i + 1) / W) ? v[i + 1] : 0.f);
         amax = row_reduce<true>(amax, tpr, slot);
-        const float s = fmaxf(__fdiv_rn(amax, 127.0f), 1.0e-30f), inv = __frcp_rn(s);
+        const float s = max_nan(__fdiv_rn(amax, 127.0f), 1.0e-30f), inv = __frcp_rn(s);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             if constexpr (W == 1) {
@@ -513,9 +526,9 @@ __global__ void __launch_bounds__(kFlatThreads, 1) residual_norm_flat_kernel(con
             row.clear(x);
             float amax = 0.f;
 #pragma unroll
-            for (int i = 0; i < kFlatVpt; ++i) amax = fmaxf(amax, fabsf(x[i]));
+            for (int i = 0; i < kFlatVpt; i += 2) amax = max_size_nan(amax, x[i], x[i + 1]);
             amax = row_reduce<true>(amax, TPR, slots + 4 * SL);
-            const float s = fmaxf(__fdiv_rn(amax, 127.0f), 1.0e-30f), inv = __frcp_rn(s);
+            const float s = max_nan(__fdiv_rn(amax, 127.0f), 1.0e-30f), inv = __frcp_rn(s);
             int8_t *const q = a.q + (long long)m * a.ldq;
 #pragma unroll
             for (int c = 0; c < kFlatGroups; ++c) {

@@ -383,7 +383,8 @@ def residual_norm_quantized(x: Tensor, y: Tensor, *, post_norm=None, gate: Tenso
                             scale: float = 1.0, pre_norm=None, out: Tensor | None = None,
                             pdl: bool = False) -> tuple[Tensor, Tensor, Tensor]:
     """residual_norm with the next 8-bit projection's quantizer in the same pass -> (r, q, qs): q INT8 [m, D] codes of h's
-    rows (held 16-byte aligned) with one FP32 scale each, qs [m], as quantize() forms one part. h is never written."""
+    rows (held 16-byte aligned) with one FP32 scale each, qs [m], as quantize() forms one part; but a row of h that holds a
+    NaN has scale NaN (quantize() passes a NaN by), so what is multiplied with it is not a number. h is never written."""
     return (_lib._native or _lib.native()).residual_norm_quantized(x, y, post_norm, gate, gate_act, scale, pre_norm, out,
                                                                    pdl)
 

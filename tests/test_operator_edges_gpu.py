@@ -8,6 +8,7 @@ import ctypes
 
 import pytest
 import torch
+from torch import nn
 
 from kea_kernels import _lib, lowbit
 from test_operators_cpu import ResidualNormDesc
@@ -173,3 +174,25 @@ def test_a_bias_beside_root_mean_square_norms(rows, d):
     want_h = norm(want_r, w2, b2)
     for got, want in ((r, want_r), (h, want_h)):
         assert bool(((got.double() - want).abs() <= 3e-5 * want.abs().amax(-1, keepdim=True).clamp_min(1.0)).all())
+
+
+@pytest.mark.parametrize("rows,d", [(9, 64), (9, 65), (12024, 1001), (4000, 1024)])
+@pytest.mark.parametrize("norm", [None, nn.LayerNorm, nn.RMSNorm])
+def test_a_row_that_is_not_a_number_has_no_scale(rows, d, norm):
+    """INT8 codes hold no NaN, so the row's scale does: the 8-bit map after it returns NaN for that row, as it would in FP32,
+    and leaves the others as they were. An infinity gives NaN too (its codes are relative to an infinite scale)."""
+    gen = torch.Generator(device=DEV).manual_seed(d)
+    x, y = (torch.randn(1, rows, d, generator=gen, device=DEV) for _ in range(2))
+    pre = None if norm is None else norm(d, eps=1e-5).to(DEV)
+    w = torch.randint(-127, 128, (32, -(-d // 16) * 16), generator=gen, device=DEV).to(torch.int8)
+    alpha = torch.rand(32, generator=gen, device=DEV)
+    run = lambda: (lambda r, q, qs: (q, qs, lowbit.int8_linear(q, qs, w, alpha, k=d)))(  # noqa: E731
+        *lowbit.residual_norm_quantized(x, y, pre_norm=pre))
+    q, qs, out = run()
+    assert bool(qs.isfinite().all()) and bool(out.isfinite().all())
+    y[0, 2, d // 2], x[0, 5, d - 1], y[0, rows - 1, 0] = float("nan"), float("nan"), float("inf")
+    q2, qs2, out2 = run()
+    bad = torch.zeros(rows, dtype=torch.bool, device=DEV)
+    bad[[2, 5, rows - 1]] = True
+    assert bool(qs2[[2, 5]].isnan().all()) and bool(out2[bad].isnan().all())
+    assert torch.equal(q2[~bad], q[~bad]) and torch.equal(qs2[~bad], qs[~bad]) and torch.equal(out2[~bad], out[~bad])
