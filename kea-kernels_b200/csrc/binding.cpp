@@ -30,6 +30,7 @@ struct Library {
     decltype(&kea_lowbit_beam_reorder) beam_reorder = nullptr;
     decltype(&kea_lowbit_status_string) status_string = nullptr;
     PyObject *layer_norm = nullptr, *rms_norm = nullptr;   // nn.LayerNorm, nn.RMSNorm
+    PyObject *layer_forward = nullptr, *rms_forward = nullptr;
 } lib;
 
 [[noreturn]] void raise(PyObject *type, const std::string &text) {
@@ -214,7 +215,8 @@ struct Norm {
     const float *weight = nullptr, *bias = nullptr;
 };
 
-// An nn.LayerNorm or nn.RMSNorm over the last dimension, or None.
+// An nn.LayerNorm or nn.RMSNorm over the last dimension, or None. The module is read, not called, so one whose call would do
+// something else - a class with a forward of its own, a forward or hooks of the module's - is refused.
 Norm norm_of(PyObject *o, int64_t d, const at::Device &device, const char *name) {
     Norm r;
     if (none(o)) return r;
@@ -225,6 +227,22 @@ Norm norm_of(PyObject *o, int64_t d, const at::Device &device, const char *name)
     r.kind = layer ? KEA_NORM_LAYER : KEA_NORM_RMS;
     static PyObject *const s_parameters = PyUnicode_InternFromString("_parameters"), *const s_eps = PyUnicode_InternFromString("eps");
     static PyObject *const s_weight = PyUnicode_InternFromString("weight"), *const s_bias = PyUnicode_InternFromString("bias");
+    static PyObject *const s_forward = PyUnicode_InternFromString("forward");
+    static PyObject *const s_hooks[2] = {PyUnicode_InternFromString("_forward_hooks"), PyUnicode_InternFromString("_forward_pre_hooks")};
+    PyObject *const type = reinterpret_cast<PyObject *>(Py_TYPE(o));
+    if (type != (layer ? lib.layer_norm : lib.rms_norm)) {
+        THPObjectPtr forward(PyObject_GetAttr(type, s_forward));
+        if (!forward) throw python_error();
+        if (forward.get() != (layer ? lib.layer_forward : lib.rms_forward)) refuse(std::string(name) + "'s class has a forward of its own");
+    }
+    THPObjectPtr own(PyObject_GenericGetDict(o, nullptr));
+    if (!own) throw python_error();
+    if (PyDict_GetItemWithError(own.get(), s_forward)) refuse(std::string(name) + " has a forward of its own");
+    for (PyObject *s : s_hooks) {
+        PyObject *hooks = PyDict_GetItemWithError(own.get(), s);   // borrowed
+        if (hooks && PyDict_Check(hooks) && PyDict_Size(hooks) > 0) refuse(std::string(name) + " has forward hooks, which would not run");
+    }
+    if (PyErr_Occurred()) throw python_error();
     THPObjectPtr parameters(PyObject_GetAttr(o, s_parameters)), eps(PyObject_GetAttr(o, s_eps));
     if (!parameters || !eps) throw python_error();
     if (!PyDict_Check(parameters.get())) refuse(std::string(name) + " must be a module with parameters");
@@ -529,6 +547,9 @@ PyObject *bind(PyObject *, PyObject *const *o, Py_ssize_t n_args) {
     lib.status_string = reinterpret_cast<decltype(lib.status_string)>(address[4]);
     Py_XSETREF(lib.layer_norm, Py_NewRef(o[5]));
     Py_XSETREF(lib.rms_norm, Py_NewRef(o[6]));
+    Py_XSETREF(lib.layer_forward, PyObject_GetAttrString(o[5], "forward"));
+    Py_XSETREF(lib.rms_forward, PyObject_GetAttrString(o[6], "forward"));
+    if (!lib.layer_forward || !lib.rms_forward) throw python_error();
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }

@@ -372,10 +372,10 @@ def residual_norm(x: Tensor, y: Tensor, *, post_norm=None, gate: Tensor | None =
                   pdl: bool = False) -> tuple[Tensor, Tensor]:
     """The step between two blocks in one pass: r = x + scale * act(gate) * post_norm(y), h = pre_norm(r) -> (r, h).
     x [..., T, D] is the residual stream, y the block's output (each FP32, FP16 or BF16, rows at one stride); post_norm and
-    pre_norm are nn.LayerNorm / nn.RMSNorm modules or None; gate (y's type) is one row [D], one row per clip [B, D] of
-    x [B, T, D], or of x's shape, taken as it is or through the logistic function (gate_act "sigmoid"). r has x's type
-    (written to `out` where given, x itself included) and h `dtype` (y's by default). h is the norm of r before its
-    rounding; all arithmetic is FP32."""
+    pre_norm are nn.LayerNorm / nn.RMSNorm modules or None, which are read, not called: a forward of their own or forward
+    hooks are refused; gate (y's type) is one row [D], one row per clip [B, D] of x [B, T, D], or of x's shape, taken as it is
+    or through the logistic function (gate_act "sigmoid"). r has x's type (written to `out` where given, x itself included)
+    and h `dtype` (y's by default). h is the norm of r before its rounding; all arithmetic is FP32."""
     return (_lib._native or _lib.native()).residual_norm(x, y, post_norm, gate, gate_act, scale, pre_norm, out, pdl, dtype)
 
 

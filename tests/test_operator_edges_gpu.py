@@ -196,3 +196,33 @@ def test_a_row_that_is_not_a_number_has_no_scale(rows, d, norm):
     bad[[2, 5, rows - 1]] = True
     assert bool(qs2[[2, 5]].isnan().all()) and bool(out2[bad].isnan().all())
     assert torch.equal(q2[~bad], q[~bad]) and torch.equal(qs2[~bad], qs[~bad]) and torch.equal(out2[~bad], out[~bad])
+
+
+def test_norms_with_a_forward_of_their_own_are_refused():
+    """A norm is read, not called: a class or a module that computes something else, or hooks that would run, are turned
+    away; a class that only bears another name is taken."""
+    class PlusOne(nn.LayerNorm):
+        def forward(self, v):
+            return nn.functional.layer_norm(v, self.normalized_shape, self.weight + 1, self.bias, self.eps)
+
+    class Named(nn.RMSNorm):
+        pass
+
+    d = 64
+    x, y = torch.randn(2, 3, d, device=DEV), torch.randn(2, 3, d, device=DEV)
+    own, hooked, before, replaced = PlusOne(d).to(DEV), nn.LayerNorm(d).to(DEV), nn.RMSNorm(d).to(DEV), nn.LayerNorm(d).to(DEV)
+    hooked.register_forward_hook(lambda module, args, out: 2 * out)
+    before.register_forward_pre_hook(lambda module, args: (2 * args[0],))
+    replaced.forward = lambda v: v
+    for bad in (own, hooked, before, replaced):
+        for option in ("post_norm", "pre_norm"):
+            with pytest.raises(ValueError):
+                lowbit.residual_norm(x, y, **{option: bad})
+            with pytest.raises(ValueError):
+                lowbit.residual_norm_quantized(x, y, **{option: bad})
+    handle = replaced.register_forward_hook(lambda module, args, out: out)
+    del replaced.forward
+    handle.remove()
+    for fine, like in ((Named(d, eps=1e-6).to(DEV), nn.RMSNorm(d, eps=1e-6).to(DEV)), (replaced, nn.LayerNorm(d).to(DEV))):
+        for a, b in zip(lowbit.residual_norm(x, y, pre_norm=fine), lowbit.residual_norm(x, y, pre_norm=like)):
+            assert torch.equal(a, b)
