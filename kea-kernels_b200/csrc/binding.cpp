@@ -4,6 +4,7 @@
 // microseconds on the GPU and filling a descriptor through ctypes would take several times that on the host.
 // The C-ABI functions are handed over by address at import (bind), so that one loaded library serves every caller.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -15,6 +16,7 @@
 #include <cstring>
 #include <limits>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "kea_lowbit.h"
@@ -465,6 +467,59 @@ Layout layout(const Tensor &t, int64_t batch, const char *what, Py_ssize_t index
     return r;
 }
 
+// The bytes of a state or an output: rows at three strides.
+struct Span {
+    uintptr_t first, end;
+    int64_t row, rows;
+    int64_t count[3], step[3];
+    Span(const void *p, const Layout &l, int64_t clips, int64_t beams)
+        : first(reinterpret_cast<uintptr_t>(p)), end(first + l.row), row(l.row), rows(l.groups * clips * beams), count{l.groups, clips, beams},
+          step{l.group, l.clip, l.beam} {
+        for (int i = 0; i < 3; ++i) {
+            if (count[i] == 1) step[i] = 0;
+            end += (count[i] - 1) * step[i];
+        }
+    }
+    // From the first byte to the last, modulo s: steps that are its multiples do not count.
+    int64_t extent(int64_t s) const {
+        int64_t n = row;
+        for (int i = 0; i < 3; ++i)
+            if (step[i] % s) n += (count[i] - 1) * step[i];
+        return n;
+    }
+    void add(std::vector<std::pair<uintptr_t, uintptr_t>> &to) const {
+        for (int64_t g = 0; g < count[0]; ++g)
+            for (int64_t b = 0; b < count[1]; ++b)
+                for (int64_t k = 0; k < count[2]; ++k) {
+                    const uintptr_t at = first + g * step[0] + b * step[1] + k * step[2];
+                    to.emplace_back(at, at + row);
+                }
+    }
+};
+
+// Whether no byte is in both: by their ends, by one of the steps (halves of a buffer that interleave), or row by row.
+bool apart(const Span &a, const Span &b) {
+    if (a.end <= b.first || b.end <= a.first) return true;
+    for (const Span *of : {&a, &b})
+        for (const int64_t s : of->step) {
+            if (s == 0) continue;
+            const int64_t from = ((int64_t)(b.first - a.first) % s + s) % s, ea = a.extent(s), eb = b.extent(s);
+            if (from >= ea && from + eb <= s) return true;
+        }
+    if (a.rows + b.rows > (1 << 22)) return false;   // taken for an overlap
+    std::vector<std::pair<uintptr_t, uintptr_t>> ra, rb;
+    a.add(ra);
+    b.add(rb);
+    std::sort(ra.begin(), ra.end());
+    std::sort(rb.begin(), rb.end());
+    for (size_t i = 0, j = 0; i < ra.size() && j < rb.size();) {
+        if (ra[i].second <= rb[j].first) ++i;
+        else if (rb[j].second <= ra[i].first) ++j;
+        else return false;
+    }
+    return true;
+}
+
 // (states, parents, batch_dim, out or None, pdl, error_word) -> list
 PyObject *beam_reorder(PyObject *, PyObject *const *o, Py_ssize_t n_args) {
     HANDLE_TH_ERRORS
@@ -493,6 +548,7 @@ PyObject *beam_reorder(PyObject *, PyObject *const *o, Py_ssize_t n_args) {
     THPObjectPtr results(PyList_New(total));
     if (!results) throw python_error();
     std::vector<KeaReorderItem> items;
+    std::vector<Span> read, written;   // with outputs given
     items.reserve((size_t)total);
     int64_t beams = -1;
     for (Py_ssize_t i = 0; i < total; ++i) {
@@ -511,16 +567,28 @@ PyObject *beam_reorder(PyObject *, PyObject *const *o, Py_ssize_t n_args) {
             r = tensor(PySequence_Fast_GET_ITEM(given.get(), i), "an output");
             if (r.sizes() != at::IntArrayRef(want) || r.scalar_type() != s.scalar_type() || r.device() != device)
                 refuse("output " + std::to_string(i) + " must have its state's type and shape with " + std::to_string(width) + " places");
-            if (r.numel() && r.const_data_ptr() == s.const_data_ptr()) refuse("output " + std::to_string(i) + " may not be the state itself");
+            if (at::has_internal_overlap(r) == at::MemOverlap::Yes) refuse("output " + std::to_string(i) + " overlaps itself");
         }
         if (r.numel()) {
             const Layout from = layout(s, batch, "state", i), into = layout(r, batch, "output", i);
             items.push_back(KeaReorderItem{s.const_data_ptr(), r.data_ptr(), from.group, from.clip, from.beam, into.group, into.clip,
                                            into.beam, from.row, small(from.groups, "a state")});
+            if (given) {
+                read.emplace_back(s.const_data_ptr(), from, clips, beams);
+                written.emplace_back(r.data_ptr(), into, clips, width);
+            }
         }
         PyObject *wrapped = given ? Py_NewRef(PySequence_Fast_GET_ITEM(given.get(), i)) : THPVariable_Wrap(std::move(r));
         if (!wrapped) throw python_error();
         PyList_SET_ITEM(results.get(), i, wrapped);
+    }
+    // every row moves in one launch, in any order
+    if (!written.empty()) read.emplace_back(parents.const_data_ptr(), Layout{0, 0, 0, (int64_t)parents.nbytes(), 1}, 1, 1);
+    for (size_t i = 0; i < written.size(); ++i) {
+        for (const Span &from : read)
+            if (!apart(written[i], from)) refuse("an output overlaps a state or the parents");
+        for (size_t j = 0; j < i; ++j)
+            if (!apart(written[i], written[j])) refuse("two outputs overlap");
     }
     d.beams = small(std::max<int64_t>(beams, 1), "a state");
     for (size_t first = 0; first < items.size(); first += KEA_REORDER_MAX) {

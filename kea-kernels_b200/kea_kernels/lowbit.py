@@ -417,6 +417,6 @@ def beam_reorder(states: Sequence[Tensor], parents: Tensor, *, batch_dim: int = 
     """The states of a beam search's chosen hypotheses: for every state [..., clips, beams, ...] (clips and beams at
     dimensions batch_dim and batch_dim + 1; what follows them contiguous, the dimensions before them at one stride)
     result[..., b, w, ...] = state[..., b, parents[b, w], ...], all states in one launch. parents int32 [clips, width].
-    `out`: tensors to write to, not the states themselves. A parent outside the hypotheses leaves zeros and sets
-    DEVERR_INDEX in the error word."""
+    `out`: tensors to write to, of which none may share memory with a state, the parents or another one (halves of a buffer
+    that interleave are fine). A parent outside the hypotheses leaves zeros and sets DEVERR_INDEX in the error word."""
     return (_lib._native or _lib.native()).beam_reorder(states, parents, batch_dim, out, pdl, error_word)

@@ -226,3 +226,28 @@ def test_norms_with_a_forward_of_their_own_are_refused():
     for fine, like in ((Named(d, eps=1e-6).to(DEV), nn.RMSNorm(d, eps=1e-6).to(DEV)), (replaced, nn.LayerNorm(d).to(DEV))):
         for a, b in zip(lowbit.residual_norm(x, y, pre_norm=fine), lowbit.residual_norm(x, y, pre_norm=like)):
             assert torch.equal(a, b)
+
+
+def test_reorder_refuses_outputs_that_overlap():
+    """All states move in one launch: an output may share no byte with any state, nor with another output or itself.
+    Buffers that only interleave are taken."""
+    clips, beams = 3, 4
+    parents = torch.tensor([[1, 0, 3, 2], [0, 0, 2, 1], [3, 3, 3, 0]], device=DEV, dtype=torch.int32)
+    make = lambda *shape: torch.randn(*shape, device=DEV)  # noqa: E731
+    a, b, free = make(clips, beams, 8), make(clips, beams, 8), make(clips, beams, 8)
+    flat, pair, wide = make(clips * beams * 8 + 8), make(clips, beams, 2, 8), make(clips, beams, 12)
+    shifted = [flat[i:i + clips * beams * 8].view(clips, beams, 8) for i in (0, 8)]
+    call = lowbit.beam_reorder
+    for states, out in (([a, b], [b, a]), ([a, b], [free, a]), ([a], [a]), (shifted[:1], shifted[1:]), (shifted[1:], shifted[:1]),
+                        ([a, b], [free, free]), ([a], [make(8).expand(clips, beams, 8)]), ([wide[..., :8]], [wide[..., 4:]]),
+                        ([pair[:, :, 0]], [pair.view(clips, 2, beams, 8)[:, 1]]), ([a], [a.view(beams, clips, 8).transpose(0, 1)])):
+        with pytest.raises(ValueError):
+            call(states, parents, out=out)
+    row = torch.arange(clips, device=DEV)[:, None]
+    layers, halves = make(clips, 2, beams, 8), make(2, 3, clips, beams, 5)
+    for states, out, batch in (([pair[:, :, 0]], [pair[:, :, 1]], 0), ([layers[:, 1]], [layers[:, 0]], 0), ([halves[0]], [halves[1]], 1),
+                               ([halves[:, 0], halves[:, 1]], [halves[:, 2], make(2, clips, beams, 5)], 1), ([a, a], [b, free], 0),
+                               ([wide[..., :6]], [wide[..., 6:]], 0)):
+        want = [s[row, parents.long()] if batch == 0 else s[:, row, parents.long()] for s in states]
+        for got, o, w in zip(call(states, parents, batch_dim=batch, out=out), out, want):
+            assert got is o and torch.equal(got, w)
