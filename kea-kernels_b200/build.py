@@ -74,20 +74,40 @@ def run(cmd: list[str]) -> str:
     return res.stderr
 
 
+def build_library() -> str:
+    """Compiles the sources side by side into a temporary folder and links them."""
+    with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(len(SOURCES)) as pool:
+        objects = [Path(tmp) / f"{s.stem}.o" for s in SOURCES]
+        logs = list(pool.map(run, map(compile_command, SOURCES, objects)))
+        return "".join([*logs, run(link_command(objects))])
+
+
+def build_binding() -> str:
+    """Compiles the extension. Without torch there is no Python side to serve, and the library stands alone."""
+    try:
+        command = binding_command()
+    except ModuleNotFoundError as e:
+        if e.name != "torch":
+            raise
+        print("torch is not installed: only the C library is built", file=sys.stderr)
+        return ""
+    return run(command)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compiles the sources side by side into a temporary folder and links them; the binding beside them."""
+    """The library, which needs nvcc alone, and the binding beside it. A binding that does not build is an error, after the
+    library has been put in its place."""
     library, binding = force or stale(), force or binding_stale()
-    with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(len(SOURCES) + 1) as pool:
-        extension = pool.submit(run, binding_command()) if binding else None
-        logs = []
-        if library:
-            objects = [Path(tmp) / f"{s.stem}.o" for s in SOURCES]
-            logs = list(pool.map(run, map(compile_command, SOURCES, objects)))
-            logs.append(run(link_command(objects)))
+    with ThreadPoolExecutor(1) as pool:
+        extension = pool.submit(build_binding) if binding else None
+        log = build_library() if library else ""
         if extension is not None:
-            logs.append(extension.result())
+            try:
+                log += extension.result()
+            except Exception as e:
+                raise RuntimeError(f"{OUT.name} is built, {BINDING.name} (the Python entry points) is not: {e}") from e
     if verbose:
-        print("".join(logs))
+        print(log)
     return OUT
 
 
