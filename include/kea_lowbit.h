@@ -350,8 +350,9 @@ typedef struct KeaInt8Desc {
 
 enum {
     KEA_INT8_SILU = 1,
-    KEA_INT8_PDL = 2              /* launch with programmatic dependent launch; the weights may be read before the previous
-                                     kernel of the stream has ended, so that kernel may not write them */
+    KEA_INT8_PDL = 2              /* launch with programmatic dependent launch; the weights may be read before earlier kernels of
+                                     the stream have ended: neither the previous kernel nor, where that was launched this
+                                     way too, one before it may write them */
 };
 enum {
     KEA_INT8_KERNEL_REG = 1,      /* warp-level MMAs on operands loaded straight into registers: few tokens */

@@ -42,6 +42,8 @@ class Int8Linear(nn.Module):
         self.register_buffer("panels", codes.as_strided((codes.shape[0], codes.stride(0)), codes.stride()))
         self.register_buffer("scale", scale)
         self.register_buffer("bias", None if bias is None else bias.detach().to(device=device, dtype=torch.float32).contiguous())
+        if device.type == "cuda":   # the product may read its weights before earlier kernels of its stream have ended
+            torch.cuda.current_stream(device).synchronize()
 
     def product(self, q: Tensor, qs: Tensor, *, silu: bool = False, residual: Tensor | None = None,
                 residual_scale: float = 1.0, dtype: torch.dtype = torch.float32, pdl: bool | None = None) -> Tensor:

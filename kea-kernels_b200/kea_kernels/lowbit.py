@@ -362,7 +362,8 @@ def int8_linear(q: Tensor, qs: Tensor, weight: Tensor, alpha: Tensor, bias: Tens
     scales, bias FP32 [n], SiLU and residual + residual_scale * value, each one FP32 rounding -> [m, n] of `dtype` (FP32,
     FP16 or BF16), or `out` (unit column stride) where given. residual: [m, n] of the output's type, unit column stride; may
     be `out` itself. Rows of q and weight are 16-byte aligned; with `k`, columns >= k of both are ignored. acc (INT32
-    [m, n], unit column stride) receives the sums. kernel forces one of INT8_KERNEL_* (0: chosen by the shape)."""
+    [m, n], unit column stride) receives the sums. kernel forces one of INT8_KERNEL_* (0: chosen by the shape). pdl lets the
+    kernel start, and read `weight`, while earlier kernels of the stream finish: none of those may still be writing it."""
     return (_lib._native or _lib.native()).int8_linear(q, qs, weight, alpha, bias, out, k, dtype, silu, residual,
                                                        residual_scale, acc, kernel, pdl, error_word)
 
@@ -375,7 +376,8 @@ def residual_norm(x: Tensor, y: Tensor, *, post_norm=None, gate: Tensor | None =
     pre_norm are nn.LayerNorm / nn.RMSNorm modules or None, which are read, not called: a forward of their own or forward
     hooks are refused; gate (y's type) is one row [D], one row per clip [B, D] of x [B, T, D], or of x's shape, taken as it is
     or through the logistic function (gate_act "sigmoid"). r has x's type (written to `out` where given, x itself included)
-    and h `dtype` (y's by default). h is the norm of r before its rounding; all arithmetic is FP32."""
+    and h `dtype` (y's by default). h is the norm of r before its rounding; all arithmetic is FP32. pdl: as for
+    int8_linear, with the norms' parameters in the weights' place."""
     return (_lib._native or _lib.native()).residual_norm(x, y, post_norm, gate, gate_act, scale, pre_norm, out, pdl, dtype)
 
 

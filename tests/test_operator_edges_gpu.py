@@ -11,6 +11,7 @@ import torch
 from torch import nn
 
 from kea_kernels import _lib, lowbit
+from kea_kernels.int8 import Int8Linear
 from test_operators_cpu import ResidualNormDesc
 
 pytestmark = pytest.mark.gpu
@@ -251,3 +252,14 @@ def test_reorder_refuses_outputs_that_overlap():
         want = [s[row, parents.long()] if batch == 0 else s[:, row, parents.long()] for s in states]
         for got, o, w in zip(call(states, parents, batch_dim=batch, out=out), out, want):
             assert got is o and torch.equal(got, w)
+
+
+def test_weights_are_complete_when_a_layer_is():
+    """A layer's product is launched so that it may read the weights while earlier kernels finish; they must not be among
+    what those write. The wait keeps the stream busy for some 50 ms before the weights' kernels."""
+    weight = torch.randn(256, 128, device=DEV)
+    Int8Linear(weight)   # what loads at a first use has loaded
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)
+    Int8Linear(weight)
+    assert torch.cuda.current_stream().query()
