@@ -62,6 +62,8 @@ class BeamDecoder(nn.Module):
         """enc FP32 [B, T, d_model] (with `lengths`, int [B]: frames of each clip, the rest is padding) -> the `width` best
         hypotheses of every clip. Past a clip's end its hypotheses have ended: they add blanks at no cost."""
         b, t, _ = enc.shape
+        if lengths is not None and tuple(lengths.shape) != (b,):
+            raise ValueError(f"lengths must be [{b}], got {tuple(lengths.shape)}")
         device, blank = enc.device, self.blank
         frames = self.enc(enc)
         labels = torch.full((t, b, width), blank, device=device, dtype=torch.int32)

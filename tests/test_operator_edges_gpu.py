@@ -11,6 +11,7 @@ import torch
 from torch import nn
 
 from kea_kernels import _lib, lowbit
+from kea_kernels.decoder import BeamDecoder
 from kea_kernels.int8 import Int8Linear
 from test_operators_cpu import ResidualNormDesc
 
@@ -263,3 +264,15 @@ def test_weights_are_complete_when_a_layer_is():
     torch.cuda._sleep(100_000_000)
     Int8Linear(weight)
     assert torch.cuda.current_stream().query()
+
+
+def test_search_refuses_lengths_of_other_clips():
+    """One length for three clips would otherwise end all of them there; no clips and no frames are searches too."""
+    dec = BeamDecoder(d_model=32, hidden=32, vocab=10, device=DEV)
+    enc = torch.randn(3, 4, 32, device=DEV)
+    for lengths in (torch.tensor([2]), torch.tensor(2), torch.tensor([[4], [4], [4]]), torch.tensor([4, 4])):
+        with pytest.raises(ValueError):
+            dec.search(enc, lengths, 2)
+    for some in (enc[:0], enc[:, :0]):
+        found = dec.search(some, torch.full((some.shape[0],), some.shape[1]), 2)
+        assert found.labels.shape == (some.shape[0], 2, some.shape[1]) and found.scores.shape == (some.shape[0], 2)
