@@ -323,9 +323,11 @@ enum { KEA_TYPE_F32 = 0, KEA_TYPE_F16 = 1, KEA_TYPE_BF16 = 2 };
  *   acc[m, n] = sum_k q[m, k] * w[n, k]                                  (exact INT32)
  *   v         = bias ? fma(RN(acc) * qs[m], alpha[n], bias[n]) : (RN(acc) * qs[m]) * alpha[n],  then SiLU if KEA_INT8_SILU
  *   y[m, n]   = residual ? residual[m, n] + residual_scale * v : v       (FP32, rounded once to y_type)
- * with one IEEE FP32 rounding per operation, as kea_lowbit_gemm. For layers kept at 8 bits (a joint network, layers an
- * export leaves unpacked); the weights are used as they are, row-major, without a layout pass. k <= 131071, where no sum
- * can leave INT32. q and w: 16-byte aligned, row strides multiples of 16; columns >= k are never used. */
+ * with one IEEE FP32 rounding per operation, as kea_lowbit_gemm; but SiLU, v / (1 + exp(-v)), is formed with an approximate
+ * exponential and reciprocal (2e-6 relative; 0 for v below -87; not the bits of KEA_FLAG_SILU). For layers kept at 8 bits
+ * (a joint network, layers an export leaves unpacked); the weights are used as they are, row-major, without a layout pass.
+ * k <= 131071, where no sum can leave INT32. q and w: 16-byte aligned, row strides multiples of 16; columns >= k are never
+ * used. */
 typedef struct KeaInt8Desc {
     const int8_t *q;          /* [m][ldq] */
     int64_t ldq;

@@ -6,15 +6,15 @@
 // lse_k is known. One thread-block cluster serves a clip; each of its warps takes a unit (a hypothesis, or a segment of
 // one) and streams its logits once, a tile ahead, keeping
 //   * per lane a running maximum m and the sum of 2^((x - m) log2 e), in FP32: x - m is at most zero and loses nothing where
-//     it counts, at any level of the logits (masks of the type's lowest value, log-probabilities). With m log2 e rounded
-//     instead, one FMA less per value, its rounding passes the exponential's range below about -2^30. Where the sum is not
+//     it counts, at any level of the logits (masks of the type's lowest value, log-probabilities). (One FMA with m log2 e
+//     rounded saves an addition, but that rounding passes the exponential's range below about -2^30.) Where the sum is not
 //     a number - a logit that is not one beside others in a lane's tile, or +inf - the unit is summed again with its maximum
 //     known, masking what is not a number;
 //   * the maximum of every tile.
 // The width-th largest of the lane maxima of all the CTA's warps at a hypothesis bounds its best logits from below: only
 // the few tiles whose maximum reaches it are read again (from the caches), and what reaches it in them, a little more
 // than `width` values in all, enters the warp's list. (Keeping the lists up to date while streaming made every warp pay
-// for its own `width` best: 3300 instructions for 2048 logits; one clip of 8 x 131072 FP32 logits 43 us, now 24.) Candidates are
+// for its own `width` best: 3300 instructions for 2048 logits; one clip of 8 x 131072 FP32 logits 43 us, 20 so.) Candidates are
 // gathered in shared memory and enter 32 at a time: every lane counts how many candidates and list entries are ahead of
 // its own, independent comparisons.
 // The units' sums and lists meet in the first CTA of the cluster (distributed shared memory), which forms every lse_k, merges

@@ -1,6 +1,6 @@
 // int8_epilogue.cuh - what every 8-bit GEMM kernel does with an exact INT32 sum: token and channel scales, bias, SiLU,
-// skip connection, one rounding to the output type. Each operation is one IEEE FP32 rounding in the order of the
-// low-bit GEMMs' epilogue, so all kernels give the same bits.
+// skip connection, one rounding to the output type. Every kernel takes these steps in this order, so all give the same bits. But
+// for SiLU each is one IEEE FP32 rounding in the order of the low-bit GEMMs' epilogue; SiLU is this file's own.
 #pragma once
 
 #include "operator_common.cuh"
@@ -30,8 +30,9 @@ struct Int8Args {
 // The bias where there is none: r * alpha + -0 is r * alpha, its sign included.
 constexpr float kI8NoBias = -0.0f;
 
-// Two outputs before the skip connection. SiLU: y / (1 + 2^(-y log2 e)) with the hardware's approximate exponential and
-// reciprocal (2 and 1 units in the last place; a denominator above 2^126 gives 0).
+// Two outputs before the skip connection. SiLU: y times the reciprocal of 1 + 2^(-y log2 e), the hardware's approximate exponential
+// and reciprocal (2 and 1 units in the last place, subnormals as zero; a denominator above 2^126 gives 0), so that two values
+// share the packed operations. (The low-bit epilogue divides, and keeps subnormals.)
 template <bool SILU>
 KEA_DEVI uint64_t int8_values(int a0, int a1, uint64_t s, uint64_t alpha, uint64_t bias) {
     uint64_t y = fma2(mul2(pair_of(__int2float_rn(a0), __int2float_rn(a1)), s), alpha, bias);

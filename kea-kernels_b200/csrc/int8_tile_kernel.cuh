@@ -218,10 +218,6 @@ KEA_DEVI void int8_epilogue_tile(const Int8TileArgs &p, const CUtensorMap *ymap,
     }
 }
 
-// float has no 16-bit packing; never called
-template <> KEA_DEVI uint32_t pack2<float>(float, float) { return 0u; }
-template <> KEA_DEVI float2 unpack2<float>(uint32_t) { return make_float2(0.f, 0.f); }
-
 // Split tiles: this warp's 32 rows of every rank's channels to their owners' receive space, [source][128 rows][cw].
 KEA_DEVI void int8_send_sums(uint32_t taddr, uint32_t recv, int cw, int splits, uint32_t rank, int quad) {
     const int row = quad * 32 + (int)(threadIdx.x & 31);

@@ -41,6 +41,10 @@ template <> KEA_DEVI float2 unpack2<__nv_bfloat16>(uint32_t w) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
 
+// float has no 16-bit packing; there for code that names it, never called
+template <> KEA_DEVI uint32_t pack2<float>(float, float) { return 0u; }
+template <> KEA_DEVI float2 unpack2<float>(uint32_t) { return make_float2(0.f, 0.f); }
+
 constexpr long long kOpWaitBudget = 4000000000LL;   // SM clocks (about 2 s) before a wait gives up
 
 KEA_DEVI void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {

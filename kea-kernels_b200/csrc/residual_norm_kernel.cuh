@@ -35,7 +35,6 @@ struct ResidualNormArgs {
     int M, D;
 };
 
-constexpr int kRnThreads = 256;
 constexpr int kRnMaxThreads = 512;
 constexpr int kRnSlots = 5;   // group reductions of one launch
 
@@ -84,9 +83,6 @@ KEA_DEVI void put(T *p, const float *v) {
         else *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(u);
     }
 }
-// float has no 16-bit packing; never called
-template <> KEA_DEVI uint32_t pack2<float>(float, float) { return 0u; }
-template <> KEA_DEVI float2 unpack2<float>(uint32_t) { return make_float2(0.f, 0.f); }
 
 // W values as they came from memory: 16-bit types stay packed until they are used (half the registers).
 template <typename T, int W>

@@ -4,8 +4,10 @@ gated residual step per label, straight into the next projection's codes (lowbit
 continuations are chosen over hypotheses and labels (lowbit.beam_select) and the hypotheses' states follow their parents
 (lowbit.beam_reorder).
 
-Shapes are the Parakeet TDT joint's (1024 -> 640, 640 -> 640, 640 -> 1024 labels + blank + 5 durations), weights random, as
-encoder.TDTJoint's, whose greedy labels the search refines: one label per frame, blank leaving the prediction state as it is.
+Shapes are the Parakeet TDT joint's (1024 -> 640, 640 -> 640, 640 -> 1024 labels + blank + 5 durations), weights random and the
+module's own: they are not encoder.TDTJoint's, and the prediction block is a stand-in that takes a label by a gate, not the
+recogniser's LSTM. The search chooses one label per frame, blank leaving the prediction state as it is; the durations' logits
+are left aside.
 The reference decodes greedily, one clip at a time (src/kea_kernels/ternary/decoder_kernels.py:139-157).
 """
 from __future__ import annotations
